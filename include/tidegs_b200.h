@@ -2,8 +2,9 @@
  * tidegs_b200.h -- C ABI of libtidegs_b200.so, the sm_100a implementation of
  * TideGS's resident-block optimizer / materialization / write-back hot path,
  * and of the steps either side of it: touched-only gradient accumulation,
- * per-block host DMAs, block frustum culling, and the gsplat render kernels
- * (projection, SH colors, tile intersection, rasterization).
+ * per-block host DMAs, block frustum culling, the gsplat render kernels
+ * (projection, SH colors, tile intersection, rasterization), and the learned
+ * appearance operators (layer norm, gated feed-forward block, dropout).
  *
  * Conventions shared by every entry point:
  *   - Plain pointers and sizes only. Every pointer named dev_* / inside an args
@@ -790,6 +791,103 @@ typedef struct {
 /* dL/dcoeffs[n, k, c] = v_colors[n, c] Y_k; dL/ddirs through the
  * normalization (compute_sh_bwd.cu; v_dirs only when not NULL). */
 TGS_API int tgs_sh_bwd(const TgsShBwdArgs* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Learned appearance: operators over rows of per-Gaussian features that
+ * complement the SH colors (no counterpart in the reference). Tensors are
+ * row-major with unit column stride; strides count elements. Sums are in 32
+ * bits; outputs are rounded once to their tensor's type.
+ * ------------------------------------------------------------------------- */
+#define TGS_F32 0
+#define TGS_BF16 1
+#define TGS_F16 2
+
+typedef struct {
+  const void* x;       /* [n, c], type dtype */
+  const void* weight;  /* [c], type param_dtype, or NULL (ones) */
+  const void* bias;    /* [c], type param_dtype, or NULL (zeros) */
+  void* y;             /* [n, c] contiguous, type dtype (forward) */
+  int64_t n;
+  int64_t x_stride;    /* elements from row to row, >= c */
+  int32_t c;           /* 1..8192 */
+  int32_t dtype;
+  int32_t param_dtype;
+  float eps;
+} TgsLayerNormArgs;
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over each row. */
+TGS_API int tgs_layer_norm_fwd(const TgsLayerNormArgs* args, void* stream);
+
+/* Floats of scratch that tgs_layer_norm_bwd needs for the parameters'
+ * gradients. */
+TGS_API int64_t tgs_layer_norm_scratch_floats(int64_t n, int32_t c);
+
+typedef struct {
+  TgsLayerNormArgs fwd;  /* y and bias unused */
+  const void* v_y;       /* [n, c], type dtype */
+  int64_t v_y_stride;
+  void* v_x;             /* [n, c] contiguous, type dtype, or NULL */
+  void* v_weight;        /* [c], type param_dtype, or NULL */
+  void* v_bias;          /* [c], type param_dtype, or NULL */
+  float* scratch;        /* when v_weight or v_bias is given */
+} TgsLayerNormBwdArgs;
+
+/* Gradients of the layer norm; the row statistics are recomputed from x. */
+TGS_API int tgs_layer_norm_bwd(const TgsLayerNormBwdArgs* args, void* stream);
+
+typedef struct {
+  const void* x;       /* [n, d] */
+  const void* w_gate;  /* [h, d] contiguous */
+  const void* w_up;    /* [h, d] contiguous */
+  const void* w_down;  /* [o, h] contiguous */
+  void* y;             /* [n, o] contiguous (forward) */
+  int64_t n;           /* at most 2^31 */
+  int64_t x_stride;    /* elements from row to row, >= d */
+  int32_t d;           /* 1..256 */
+  int32_t h;           /* 1..4096 */
+  int32_t o;           /* 1..256 */
+  int32_t dtype;       /* TGS_F32 or TGS_BF16, of every tensor */
+} TgsFfnArgs;
+
+/* y = (silu(x w_gate^T) * (x w_up^T)) w_down^T in one kernel. */
+TGS_API int tgs_ffn_fwd(const TgsFfnArgs* args, void* stream);
+
+/* Floats of scratch that tgs_ffn_bwd needs for the weights' gradients. */
+TGS_API int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32_t o, int32_t dtype);
+
+typedef struct {
+  TgsFfnArgs fwd;      /* y unused */
+  const void* v_y;     /* [n, o] */
+  int64_t v_y_stride;
+  void* v_x;           /* [n, d] contiguous, or NULL */
+  void* v_w_gate;      /* the three weights' gradients: all or none */
+  void* v_w_up;
+  void* v_w_down;
+  float* scratch;      /* when the weights' gradients are given */
+} TgsFfnBwdArgs;
+
+/* Gradients of tgs_ffn_fwd; the hidden values are recomputed. */
+TGS_API int tgs_ffn_bwd(const TgsFfnBwdArgs* args, void* stream);
+
+typedef struct {
+  const void* x;             /* [n, c] */
+  void* y;                   /* [n, c] contiguous */
+  const int64_t* ids;        /* [n] ids that stand for the rows, or NULL: 0..n-1 */
+  const int64_t* offset_dev; /* the offset in device memory, or NULL */
+  int64_t n;
+  int64_t x_stride;          /* elements from row to row, >= c */
+  uint64_t seed;
+  double p;                  /* 0..1 */
+  uint32_t offset;           /* where offset_dev is NULL */
+  int32_t c;                 /* 1..65536 */
+  int32_t per_row;           /* 1: one decision for a whole row */
+  int32_t dtype;
+} TgsDropoutArgs;
+
+/* y = x / (1 - p) where the Philox4x32-10 word of (seed, id, column, offset)
+ * is at least floor(p 2^32), else 0. The same call on the gradient is the
+ * backward pass. */
+TGS_API int tgs_dropout(const TgsDropoutArgs* args, void* stream);
 
 #ifdef __cplusplus
 }

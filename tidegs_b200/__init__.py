@@ -15,7 +15,9 @@ Drop-in classes (same names and behaviour as the reference's):
     render.fully_fused_projection,       gsplat 1.0.0 (the engine's render path,
     render.isect_tiles, isect_offset_encode, strategies/tide_engine/engine.py:481-561)
     render.rasterize_to_pixels
-plus SelectiveSophia (no reference counterpart) and PinnedBlockPool.
+plus SelectiveSophia (no reference counterpart), PinnedBlockPool and the
+learned-appearance operators of tidegs_b200.appearance (layer_norm,
+gated_feed_forward, dropout, appearance_colors; no reference counterpart).
 
 All device work runs in libtidegs_b200.so (include/tidegs_b200.h); importing
 the package does not touch the GPU, and constructing any class that owns

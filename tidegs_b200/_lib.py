@@ -23,6 +23,9 @@ MAX_GROUPS = 16
 MAX_PEERS = 64
 PEER_HANDLE_BYTES = 64
 
+F32, BF16, F16 = 0, 1, 2
+DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
 LAYOUT_CACHE = 0
 LAYOUT_UNIFIED = 1
 
@@ -195,6 +198,34 @@ class ShBwdArgs(C.Structure):
     _fields_ = [("fwd", ShArgs), ("v_colors", _vp), ("v_coeffs", _vp), ("v_dirs", _vp)]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [("x", _vp), ("weight", _vp), ("bias", _vp), ("y", _vp), ("n", _i64),
+                ("x_stride", _i64), ("c", _i32), ("dtype", _i32), ("param_dtype", _i32),
+                ("eps", C.c_float)]
+
+
+class LayerNormBwdArgs(C.Structure):
+    _fields_ = [("fwd", LayerNormArgs), ("v_y", _vp), ("v_y_stride", _i64), ("v_x", _vp),
+                ("v_weight", _vp), ("v_bias", _vp), ("scratch", _vp)]
+
+
+class FfnArgs(C.Structure):
+    _fields_ = [("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("y", _vp),
+                ("n", _i64), ("x_stride", _i64), ("d", _i32), ("h", _i32), ("o", _i32),
+                ("dtype", _i32)]
+
+
+class FfnBwdArgs(C.Structure):
+    _fields_ = [("fwd", FfnArgs), ("v_y", _vp), ("v_y_stride", _i64), ("v_x", _vp),
+                ("v_w_gate", _vp), ("v_w_up", _vp), ("v_w_down", _vp), ("scratch", _vp)]
+
+
+class DropoutArgs(C.Structure):
+    _fields_ = [("x", _vp), ("y", _vp), ("ids", _vp), ("offset_dev", _vp), ("n", _i64),
+                ("x_stride", _i64), ("seed", C.c_uint64), ("p", C.c_double),
+                ("offset", C.c_uint32), ("c", _i32), ("per_row", _i32), ("dtype", _i32)]
+
+
 # name -> (restype, argtypes). Keep in sync with include/tidegs_b200.h.
 SIGNATURES = {
     "tgs_version": (C.c_int, []),
@@ -257,6 +288,13 @@ SIGNATURES = {
     "tgs_rasterize_bwd": (C.c_int, [C.POINTER(RasterBwdArgs), _vp]),
     "tgs_sh_fwd": (C.c_int, [C.POINTER(ShArgs), _vp]),
     "tgs_sh_bwd": (C.c_int, [C.POINTER(ShBwdArgs), _vp]),
+    "tgs_layer_norm_fwd": (C.c_int, [C.POINTER(LayerNormArgs), _vp]),
+    "tgs_layer_norm_scratch_floats": (_i64, [_i64, _i32]),
+    "tgs_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormBwdArgs), _vp]),
+    "tgs_ffn_fwd": (C.c_int, [C.POINTER(FfnArgs), _vp]),
+    "tgs_ffn_scratch_floats": (_i64, [_i64, _i32, _i32, _i32, _i32]),
+    "tgs_ffn_bwd": (C.c_int, [C.POINTER(FfnBwdArgs), _vp]),
+    "tgs_dropout": (C.c_int, [C.POINTER(DropoutArgs), _vp]),
 }
 
 _lock = threading.Lock()
@@ -312,6 +350,8 @@ KERNELS_PER_CALL = {
     # iota + the library radix sort and scan (their kernel counts depend on
     # the library version and are not counted here)
     "tgs_isect_depth_order": 1, "tgs_isect_sort_tiles": 0,
+    "tgs_layer_norm_fwd": 1, "tgs_layer_norm_bwd": 2, "tgs_ffn_fwd": 1, "tgs_ffn_bwd": 3,
+    "tgs_dropout": 1,
 }
 launch_counter = {"kernels": 0}
 
