@@ -847,13 +847,17 @@ typedef struct {
   int32_t h;           /* 1..4096 */
   int32_t o;           /* 1..256 */
   int32_t dtype;       /* TGS_F32 or TGS_BF16, of every tensor */
+  float* scratch;      /* tgs_ffn_scratch_floats(...) floats, 16-byte aligned */
+  int32_t* err;        /* error word (a wait that ran out), or NULL */
 } TgsFfnArgs;
 
 /* y = (silu(x w_gate^T) * (x w_up^T)) w_down^T in one kernel. */
 TGS_API int tgs_ffn_fwd(const TgsFfnArgs* args, void* stream);
 
-/* Floats of scratch that tgs_ffn_bwd needs for the weights' gradients. */
-TGS_API int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32_t o, int32_t dtype);
+/* Floats of scratch that tgs_ffn_fwd (backward = 0) or tgs_ffn_bwd (1) needs
+ * on the current device. */
+TGS_API int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32_t o, int32_t dtype,
+                                       int32_t backward);
 
 typedef struct {
   TgsFfnArgs fwd;      /* y unused */
@@ -863,7 +867,6 @@ typedef struct {
   void* v_w_gate;      /* the three weights' gradients: all or none */
   void* v_w_up;
   void* v_w_down;
-  float* scratch;      /* when the weights' gradients are given */
 } TgsFfnBwdArgs;
 
 /* Gradients of tgs_ffn_fwd; the hidden values are recomputed. */

@@ -212,12 +212,12 @@ class LayerNormBwdArgs(C.Structure):
 class FfnArgs(C.Structure):
     _fields_ = [("x", _vp), ("w_gate", _vp), ("w_up", _vp), ("w_down", _vp), ("y", _vp),
                 ("n", _i64), ("x_stride", _i64), ("d", _i32), ("h", _i32), ("o", _i32),
-                ("dtype", _i32)]
+                ("dtype", _i32), ("scratch", _vp), ("err", _vp)]
 
 
 class FfnBwdArgs(C.Structure):
     _fields_ = [("fwd", FfnArgs), ("v_y", _vp), ("v_y_stride", _i64), ("v_x", _vp),
-                ("v_w_gate", _vp), ("v_w_up", _vp), ("v_w_down", _vp), ("scratch", _vp)]
+                ("v_w_gate", _vp), ("v_w_up", _vp), ("v_w_down", _vp)]
 
 
 class DropoutArgs(C.Structure):
@@ -292,7 +292,7 @@ SIGNATURES = {
     "tgs_layer_norm_scratch_floats": (_i64, [_i64, _i32]),
     "tgs_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormBwdArgs), _vp]),
     "tgs_ffn_fwd": (C.c_int, [C.POINTER(FfnArgs), _vp]),
-    "tgs_ffn_scratch_floats": (_i64, [_i64, _i32, _i32, _i32, _i32]),
+    "tgs_ffn_scratch_floats": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "tgs_ffn_bwd": (C.c_int, [C.POINTER(FfnBwdArgs), _vp]),
     "tgs_dropout": (C.c_int, [C.POINTER(DropoutArgs), _vp]),
 }

@@ -21,14 +21,14 @@ Kernels: tgs_layer_norm_fwd/bwd, tgs_ffn_fwd/bwd, tgs_dropout
 from __future__ import annotations
 
 import contextlib
-from typing import Optional, Tuple, Union
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-__all__ = ["appearance_colors", "dropout", "gated_feed_forward", "layer_norm"]
+__all__ = ["appearance_colors", "check", "dropout", "gated_feed_forward", "layer_norm"]
 
 MAX_NORM_WIDTH = 8192
 MAX_FFN_WIDTH = 256
@@ -165,23 +165,53 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
 # --- gated feed-forward block --------------------------------------------------
 
-def _ffn_args(x, w_gate, w_up, w_down) -> "_lib.FfnArgs":
+_err_words: Dict[torch.device, torch.Tensor] = {}
+
+
+def _err_word(device: torch.device) -> Optional[torch.Tensor]:
+    """The device's error word (none while a capture runs that came first)."""
+    word = _err_words.get(device)
+    if word is None and not torch.cuda.is_current_stream_capturing():
+        word = _err_words[device] = torch.zeros(4, dtype=torch.int32, device=device)
+    return word
+
+
+def check(device=None) -> None:
+    """Raises if a bounded wait inside an earlier gated_feed_forward kernel on
+    `device` (default: the current one) ran out, which leaves that call's
+    results undefined. Waits for the device."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    word = _err_words.get(device)
+    if word is None:
+        return
+    torch.cuda.synchronize(device)
+    problem = _lib.decode_device_error(word.cpu().tolist())
+    if problem is not None:
+        raise RuntimeError(f"[gated_feed_forward] {problem}")
+
+
+def _ffn_args(x, w_gate, w_up, w_down, backward: bool):
+    """(arguments, scratch tensor or None); on the tensors' device."""
     a = _lib.FfnArgs()
     a.x, a.w_gate = x.data_ptr(), w_gate.data_ptr()
     a.w_up, a.w_down = w_up.data_ptr(), w_down.data_ptr()
     a.n, a.x_stride = int(x.shape[0]), _row_stride(x)
     a.d, a.h, a.o = int(w_gate.shape[1]), int(w_gate.shape[0]), int(w_down.shape[0])
     a.dtype = _lib.DTYPES[x.dtype]
-    return a
+    a.err = _lib.ptr(_err_word(x.device))
+    words = _lib.load().tgs_ffn_scratch_floats(a.n, a.d, a.h, a.o, a.dtype, int(backward))
+    scratch = torch.empty(words, dtype=torch.float32, device=x.device) if words else None
+    a.scratch = _lib.ptr(scratch)
+    return a, scratch
 
 
 def _ffn_forward(x, w_gate, w_up, w_down):
     rows = _rows(x, x.shape[-1])
     weights = [w.detach().contiguous() for w in (w_gate, w_up, w_down)]
     y = torch.empty((*x.shape[:-1], w_down.shape[0]), dtype=x.dtype, device=x.device)
-    a = _ffn_args(rows, *weights)
-    a.y = y.data_ptr()
     with _on(x.device):
+        a, _scratch = _ffn_args(rows, *weights, backward=False)
+        a.y = y.data_ptr()
         _lib.call("tgs_ffn_fwd", a, _stream(x.device))
     return y
 
@@ -203,15 +233,10 @@ class _GatedFeedForward(torch.autograd.Function):
         v_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
         v_w = [torch.empty_like(w) for w in weights] if any(need_w) else [None] * 3
         b = _lib.FfnBwdArgs()
-        b.fwd = _ffn_args(rows, *weights)
         b.v_y, b.v_y_stride, b.v_x = v_rows.data_ptr(), _row_stride(v_rows), _lib.ptr(v_x)
         b.v_w_gate, b.v_w_up, b.v_w_down = (_lib.ptr(v) for v in v_w)
         with _on(x.device):
-            if any(need_w):
-                a = b.fwd
-                words = _lib.load().tgs_ffn_scratch_floats(a.n, a.d, a.h, a.o, a.dtype)
-                scratch = torch.empty(words, dtype=torch.float32, device=x.device)
-                b.scratch = scratch.data_ptr()
+            b.fwd, _scratch = _ffn_args(rows, *weights, backward=True)
             _lib.call("tgs_ffn_bwd", b, _stream(x.device))
         return (v_x, *(v if need else None for v, need in zip(v_w, need_w)))
 

@@ -5,10 +5,10 @@
 //   dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X, dWd = dY^T H.
 // The hidden values stay on chip: the backward recomputes G and U.
 //
-// This file: products on the ordinary fp32 pipes, a tile of rows per block,
-// the hidden width in chunks of 32.
-#include "tgs_common.cuh"
-#include "tgs_vec.cuh"
+// This file: the entry points, and 32-bit tensors: products on the ordinary
+// fp32 pipes, a tile of rows per block, the hidden width in chunks of 32.
+// bf16 tensors take the tensor cores (tgs_ffn_tc.cu).
+#include "tgs_ffn.cuh"
 
 namespace tgs {
 namespace {
@@ -18,14 +18,6 @@ constexpr int kRows = 32;   // rows per tile
 constexpr int kHid = 32;    // hidden values per chunk
 constexpr int kMaxD = 256;  // also the largest O
 constexpr int kMaxH = 4096;
-
-struct FfnParams {
-  const void *x, *dy, *wg, *wu, *wd;
-  void* y;  // dx in the backward
-  float* partial;
-  int64_t n, x_stride, dy_stride;
-  int d, h, o;
-};
 
 __device__ __forceinline__ float silu_sigmoid(float g) { return 1.f / (1.f + __expf(-g)); }
 
@@ -191,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) ffn_weights_kernel(const FfnParams p
   }
   if (h0 + hid >= p.h) return;
   const int64_t hd = static_cast<int64_t>(p.h) * p.d;
-  float* out = p.partial + blockIdx.y * (2 * hd + static_cast<int64_t>(p.h) * p.o);
+  float* out = p.scratch + blockIdx.y * (2 * hd + static_cast<int64_t>(p.h) * p.o);
 #pragma unroll
   for (int j = 0; j < kCols; ++j) {
     const int c = lane + 8 * j;
@@ -257,17 +249,12 @@ int launch_weights(const FfnParams& p, int slices, cudaStream_t s) {
   return TGS_OK;
 }
 
-template <class T>
-int ffn_forward(const FfnParams& p, cudaStream_t s) {
-  return p.o <= 64 ? launch_rows<T, false, 2>(p, s) : launch_rows<T, false, 8>(p, s);
+int64_t weights_floats(int64_t n, int d, int h, int o) {
+  return ffn_slices(n, h) * static_cast<int64_t>(h) * (2 * d + o);
 }
 
 template <class T>
-int ffn_backward(const FfnParams& p, const TgsFfnBwdArgs& b, cudaStream_t s) {
-  if (p.y && p.n > 0) {
-    if (int rc = p.d <= 64 ? launch_rows<T, true, 2>(p, s) : launch_rows<T, true, 8>(p, s)) return rc;
-  }
-  if (!b.v_w_gate) return TGS_OK;
+int ffn_weights(const FfnParams& p, cudaStream_t s) {
   int slices = 0;
   if (p.n > 0) {
     slices = ffn_slices(p.n, p.h);
@@ -277,10 +264,26 @@ int ffn_backward(const FfnParams& p, const TgsFfnBwdArgs& b, cudaStream_t s) {
   }
   const int64_t all = static_cast<int64_t>(p.h) * (2 * p.d + p.o);
   ffn_weights_sum_kernel<T><<<static_cast<unsigned>(ceil_div<int64_t>(all, kThreads)), kThreads, 0, s>>>(
-      p.partial, slices, p.d, p.h, p.o, static_cast<T*>(b.v_w_gate), static_cast<T*>(b.v_w_up),
-      static_cast<T*>(b.v_w_down));
+      p.scratch, slices, p.d, p.h, p.o, static_cast<T*>(p.dwg), static_cast<T*>(p.dwu),
+      static_cast<T*>(p.dwd));
   TGS_LAUNCH_CHECK();
   return TGS_OK;
+}
+
+int ffn_backward_f32(const FfnParams& p, cudaStream_t s) {
+  if (p.y && p.n > 0) {
+    if (int rc = p.d <= 64 ? launch_rows<float, true, 2>(p, s) : launch_rows<float, true, 8>(p, s))
+      return rc;
+  }
+  return p.dwg ? ffn_weights<float>(p, s) : TGS_OK;
+}
+
+int ffn_backward_bf16(FfnParams p, cudaStream_t s) {
+  if (p.dwg) {
+    if (int rc = ffn_weights<__nv_bfloat16>(p, s)) return rc;
+  }
+  if (!p.y || p.n == 0) return TGS_OK;
+  return ffn_tc_backward(p, s);
 }
 
 int check_ffn(const TgsFfnArgs* a, const char* who) {
@@ -300,6 +303,7 @@ int check_ffn(const TgsFfnArgs* a, const char* who) {
 FfnParams ffn_params(const TgsFfnArgs& a) {
   FfnParams p{};
   p.x = a.x, p.wg = a.w_gate, p.wu = a.w_up, p.wd = a.w_down, p.y = a.y;
+  p.scratch = a.scratch, p.err = a.err;
   p.n = a.n, p.x_stride = a.x_stride, p.d = a.d, p.h = a.h, p.o = a.o;
   return p;
 }
@@ -309,19 +313,24 @@ FfnParams ffn_params(const TgsFfnArgs& a) {
 
 using namespace tgs;
 
+extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32_t o, int32_t dtype,
+                                          int32_t backward) {
+  if (n <= 0 || d <= 0 || h <= 0 || o <= 0) return 0;
+  if (!backward) return dtype == TGS_F32 ? 0 : ffn_tc_scratch_floats(n, d, h, o, false);
+  const int64_t weights = weights_floats(n, d, h, o);
+  return dtype == TGS_F32 ? weights : std::max(weights, ffn_tc_scratch_floats(n, d, h, o, true));
+}
+
 extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
   if (int rc = check_ffn(a, "tgs_ffn_fwd")) return rc;
   if (a->n == 0) return TGS_OK;
   TGS_CHECK_ARG(a->y != nullptr, "tgs_ffn_fwd: NULL pointer");
+  TGS_CHECK_ARG(a->scratch || !tgs_ffn_scratch_floats(a->n, a->d, a->h, a->o, a->dtype, 0),
+                "tgs_ffn_fwd: scratch is NULL");
   const FfnParams p = ffn_params(*a);
-  return a->dtype == TGS_F32 ? ffn_forward<float>(p, as_stream(stream))
-                             : ffn_forward<__nv_bfloat16>(p, as_stream(stream));
-}
-
-extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32_t o, int32_t dtype) {
-  (void)dtype;
-  if (n <= 0 || d <= 0 || h <= 0 || o <= 0) return 0;
-  return ffn_slices(n, h) * static_cast<int64_t>(h) * (2 * d + o);
+  cudaStream_t s = as_stream(stream);
+  if (a->dtype == TGS_BF16) return ffn_tc_forward(p, s);
+  return p.o <= 64 ? launch_rows<float, false, 2>(p, s) : launch_rows<float, false, 8>(p, s);
 }
 
 extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {
@@ -333,9 +342,11 @@ extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {
                 "tgs_ffn_bwd: the weights' gradients are all given or none");
   TGS_CHECK_ARG(a.n == 0 || (b->v_y && (b->v_x || weights)), "tgs_ffn_bwd: NULL pointer");
   TGS_CHECK_ARG(a.n <= 1 || b->v_y_stride >= a.o, "tgs_ffn_bwd: rows of v_y overlap");
-  TGS_CHECK_ARG(a.n == 0 || !weights || b->scratch, "tgs_ffn_bwd: scratch is NULL");
+  TGS_CHECK_ARG(a.scratch || !tgs_ffn_scratch_floats(a.n, a.d, a.h, a.o, a.dtype, 1),
+                "tgs_ffn_bwd: scratch is NULL");
   FfnParams p = ffn_params(a);
-  p.dy = b->v_y, p.dy_stride = b->v_y_stride, p.y = b->v_x, p.partial = b->scratch;
-  return a.dtype == TGS_F32 ? ffn_backward<float>(p, *b, as_stream(stream))
-                            : ffn_backward<__nv_bfloat16>(p, *b, as_stream(stream));
+  p.dy = b->v_y, p.dy_stride = b->v_y_stride, p.y = b->v_x;
+  p.dwg = b->v_w_gate, p.dwu = b->v_w_up, p.dwd = b->v_w_down;
+  return a.dtype == TGS_F32 ? ffn_backward_f32(p, as_stream(stream))
+                            : ffn_backward_bf16(p, as_stream(stream));
 }

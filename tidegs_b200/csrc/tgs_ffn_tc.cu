@@ -1,0 +1,579 @@
+// Gated feed-forward block in bf16 on the 5th-generation tensor cores; the
+// formulas stand in tgs_ffn.cu.
+//
+// One persistent block per SM takes tiles of 128 rows. Per chunk of 64 hidden
+// values, "first" products (G and U as one N = 128 product; in the backward
+// dH too) land in tensor memory, eight warps turn them into the hidden chunk
+// (backward: dG and dU), rounded to bf16 into shared memory, and "second"
+// products add that chunk's share to the output tile's accumulators (Y, or
+// dX). The roles are warps of their own joined by mbarriers, so loads,
+// products and the activation of different chunks run at once:
+//   warps 0-7   activation, output        warp 8   issues matrix instructions
+//   warp  9     weight blocks (bulk copies)  warps 10-11   row tiles
+// The same block of weights serves both products: as K-major operand of one
+// and as MN-major operand of the other.
+//
+// Weights stay in shared memory where they fit (then the blocks lay them out
+// themselves); else a small kernel lays them out once per call and they
+// stream through a ring of 16 KB slots, out of L2.
+#include <cuda_bf16.h>
+
+#include "tgs_ffn.cuh"
+#include "tgs_tc.cuh"
+
+namespace tgs {
+namespace {
+
+constexpr int kEpi = 256;      // activation threads
+constexpr int kLoad = 64;      // row-tile threads
+constexpr int kTcThreads = kEpi + 64 + kLoad;
+constexpr int kTile = 128;     // rows
+constexpr int kChunk = 64;     // hidden values
+constexpr int kMaxTiles = 3;   // row-tile buffers
+constexpr int kMaxSlots = 12;  // weight ring
+constexpr int kSmemBudget = 227 * 1024 - 2048;  // less alignment and barriers
+
+struct TcParams {
+  FfnParams f;
+  const uint8_t* packed;  // laid-out weights (streaming)
+  int64_t tiles;
+  int cd, co, nc;  // operand blocks of D and O, chunks of H
+  int kd, ko;      // 16-steps of D and O
+  int nx, nh, nb, slots;
+  int resident, vec_x, vec_dy, vec_y;
+  uint32_t tile_bytes, h_bytes, w_bytes;
+  uint32_t tmem_cols;
+};
+
+struct TcBars {
+  uint64_t xfull[kMaxTiles], xempty[kMaxTiles];
+  uint64_t gfull[2], gempty[2], hfull[2], hempty[2];
+  uint64_t yfull, yempty, done;
+  uint64_t wfull[kMaxSlots], wempty[kMaxSlots];
+  uint32_t tmem;
+};
+
+// --- weights in operand layout -------------------------------------------------
+// Per chunk j: cd blocks [128][64] of D's columns, rows 0-63 the chunk's rows
+// of Wg and rows 64-127 those of Wu; then (after all chunks' blocks) Wd's
+// columns of the chunk as [16 ko][64]. Zeros beyond D, H and O.
+
+__host__ __device__ __forceinline__ uint32_t wgu_offset(const TcParams& p, int j, int c) {
+  return static_cast<uint32_t>(j * p.cd + c) * kBlockBytes;
+}
+__host__ __device__ __forceinline__ uint32_t wd_offset(const TcParams& p, int j, int b) {
+  return static_cast<uint32_t>(p.nc * p.cd) * kBlockBytes + j * p.ko * 2048 + b * kBlockBytes;
+}
+
+__device__ __forceinline__ uint4 load_unit(const __nv_bfloat16* src, int64_t at, int left,
+                                           bool vec) {
+  if (left >= 8 && vec) return *reinterpret_cast<const uint4*>(src + at);
+  union {
+    uint4 q;
+    uint16_t t[8];
+  } u;
+  u.q = make_uint4(0, 0, 0, 0);
+  const uint16_t* s = reinterpret_cast<const uint16_t*>(src) + at;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) u.t[i] = s[i];
+  return u.q;
+}
+
+// 16-byte unit `e` of the laid-out weights: its value, and where it goes.
+__device__ __forceinline__ uint4 weight_unit(const TcParams& p, uint32_t e, uint32_t* offset) {
+  const FfnParams& f = p.f;
+  const uint32_t block = e >> 10, gu_blocks = p.nc * p.cd;
+  if (block < gu_blocks) {
+    const int j = block / p.cd, c = block - j * p.cd;
+    const int row = (e >> 3) & 127, unit = e & 7;
+    const int hid = j * kChunk + (row & 63), col = c * kBlockCols + unit * 8;
+    *offset = block * kBlockBytes + unit_offset(row, unit);
+    if (hid >= f.h || col >= f.d) return make_uint4(0, 0, 0, 0);
+    const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(row < 64 ? f.wg : f.wu);
+    const bool vec = f.d % 8 == 0 && aligned16(w);
+    return load_unit(w, static_cast<int64_t>(hid) * f.d + col, f.d - col, vec);
+  }
+  const uint32_t r = (e - (gu_blocks << 10)) >> 3;  // row over all chunks
+  const int j = r / (16 * p.ko), row = r - j * 16 * p.ko, unit = e & 7;
+  const int col = j * kChunk + unit * 8;
+  *offset = gu_blocks * kBlockBytes + j * p.ko * 2048 + unit_offset(row, unit);
+  if (row >= f.o || col >= f.h) return make_uint4(0, 0, 0, 0);
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(f.wd);
+  const bool vec = f.h % 8 == 0 && aligned16(w);
+  return load_unit(w, static_cast<int64_t>(row) * f.h + col, f.h - col, vec);
+}
+
+__global__ void __launch_bounds__(256) ffn_pack_kernel(const TcParams p, uint8_t* dst) {
+  const uint32_t e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= p.w_bytes / 16) return;
+  uint32_t at;
+  const uint4 v = weight_unit(p, e, &at);
+  *reinterpret_cast<uint4*>(dst + at) = v;
+}
+
+// --- waits -----------------------------------------------------------------------
+// Every wait has a limit. After one has run out, the thread records it, skips
+// its later waits and leaves with the others; the outputs are then undefined.
+struct Waits {
+  int32_t* err;
+  bool ok = true;
+  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t phase) {
+    if (ok && !mbar_wait_bounded(bar, phase & 1)) {
+      ok = false;
+      report_error(err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
+    }
+  }
+};
+
+// --- activation --------------------------------------------------------------------
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float sigmoid(float g) {
+  return fast_rcp(1.f + fast_exp2(g * -1.4426950408889634f));
+}
+
+// Writes 16 values as bf16 into units 2 g16 and 2 g16 + 1 of a block's row.
+__device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint32_t g16,
+                                              const float (&v)[16]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint4 q;
+    q.x = pack_bf16(v[8 * half + 0], v[8 * half + 1]);
+    q.y = pack_bf16(v[8 * half + 2], v[8 * half + 3]);
+    q.z = pack_bf16(v[8 * half + 4], v[8 * half + 5]);
+    q.w = pack_bf16(v[8 * half + 6], v[8 * half + 7]);
+    st_shared16(block + unit_offset(row, 2 * g16 + half), q);
+  }
+}
+
+// Row tiles -> operand blocks: kd or ko 16-steps of columns, zeros beyond the
+// matrix.
+__device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src, int64_t stride,
+                                          int64_t r0, int64_t n, int cols, int k16, bool vec,
+                                          int tid) {
+  const int units = 2 * k16;
+  for (int e = tid; e < kTile * units; e += kLoad) {
+    const int row = e / units, unit = e - row * units;
+    const bool on = r0 + row < n && unit * 8 < cols;
+    const uint32_t at = dst + (unit >> 3) * kBlockBytes + unit_offset(row, unit & 7);
+    const int64_t from = on ? (r0 + row) * stride + unit * 8 : 0;
+    if (vec) {
+      cp_async16(at, src + from, on);
+    } else {
+      st_shared16(at, on ? load_unit(src, from, cols - unit * 8, false) : make_uint4(0, 0, 0, 0));
+    }
+  }
+}
+
+__device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, int64_t tile,
+                                             int out, int half, int lane_row) {
+  __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.f.y);
+  const int64_t row = tile * kTile + lane_row;
+  for (int c = half * 16; c < out; c += 32) {
+    float v[16];
+    tmem_ld16(acc + c, v);
+    tmem_wait_ld(v);
+    __nv_bfloat16* dst = y + row * out + c;
+    if (row >= p.f.n) {
+    } else if (p.vec_y) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (c + 8 * u < out) {
+          uint4 q;
+          q.x = pack_bf16(v[8 * u + 0], v[8 * u + 1]);
+          q.y = pack_bf16(v[8 * u + 2], v[8 * u + 3]);
+          q.z = pack_bf16(v[8 * u + 4], v[8 * u + 5]);
+          q.w = pack_bf16(v[8 * u + 6], v[8 * u + 7]);
+          *reinterpret_cast<uint4*>(dst + 8 * u) = q;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < out) dst[i] = __float2bfloat16_rn(v[i]);
+    }
+    __syncwarp();  // the next load is the whole warp's
+  }
+}
+
+// --- rows: Y, or dX --------------------------------------------------------------
+template <bool kBwd>
+__global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const TcParams p) {
+  extern __shared__ uint8_t raw[];
+  __shared__ TcBars bars;
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t xs = base;                             // nx tiles: X blocks, then dY blocks
+  const uint32_t hs = xs + p.nx * p.tile_bytes;         // nh hidden buffers
+  const uint32_t ws = hs + p.nh * p.h_bytes;            // weights, or the ring
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mine = static_cast<int>((p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  const int steps = mine * p.nc;  // n <= 2^31 and H <= 4096: below 2^30 of them
+  const int wblocks = (p.ko + 7) / 8;  // blocks of Wd per chunk
+  constexpr uint32_t kGCols = kBwd ? 192 : 128;
+  Waits wait{p.f.err};
+
+  if (warp == 8) {
+    tmem_alloc(&bars.tmem, p.tmem_cols);
+    if (lane == 0) {
+      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], kLoad), mbar_init(&bars.xempty[i], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], kEpi);
+        mbar_init(&bars.hfull[i], kEpi), mbar_init(&bars.hempty[i], 1);
+      }
+      mbar_init(&bars.yfull, 1), mbar_init(&bars.yempty, kEpi), mbar_init(&bars.done, 1);
+      for (int i = 0; i < kMaxSlots; ++i) mbar_init(&bars.wfull[i], 1), mbar_init(&bars.wempty[i], 1);
+      fence_mbar_init();
+    }
+  }
+  if (p.resident) {
+    for (uint32_t e = threadIdx.x; e < p.w_bytes / 16; e += kTcThreads) {
+      uint32_t at;
+      const uint4 v = weight_unit(p, e, &at);
+      st_shared16(ws + at, v);
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const uint32_t yacc = tmem + p.nb * kGCols;
+
+  if (warp < 8) {
+    // Activation: this thread's row of the tile, 16-column granules half,
+    // half + 2 of the chunk.
+    const uint32_t row = (warp & 3) * 32 + lane;
+    const int half = warp >> 2;
+    const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane 32 (warp % 4)
+    int j = 0;
+    int64_t tile = blockIdx.x;
+    const int out = kBwd ? p.f.d : p.f.o;
+    for (int it = 0; it < steps; ++it) {
+      const int b = p.nb == 2 ? it & 1 : 0, hb = p.nh == 2 ? it & 1 : 0;
+      wait(&bars.gfull[b], p.nb == 2 ? it >> 1 : it);
+      tc_fence_after();
+      const uint32_t acc = tmem + b * kGCols + quarter;
+      const int grans = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
+      float g[2][16], u[2][16], dh[2][16];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (half + 2 * q < grans) {
+          tmem_ld16(acc + (half + 2 * q) * 16, g[q]);
+          tmem_ld16(acc + 64 + (half + 2 * q) * 16, u[q]);
+          if constexpr (kBwd) tmem_ld16(acc + 128 + (half + 2 * q) * 16, dh[q]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        tmem_wait_ld(g[q]);
+        tmem_wait_ld(u[q]);
+        if constexpr (kBwd) tmem_wait_ld(dh[q]);
+      }
+      tc_fence_before();
+      mbar_arrive(&bars.gempty[b]);
+      if (it >= p.nh) wait(&bars.hempty[hb], p.nh == 2 ? (it >> 1) - 1 : it - 1);
+      const uint32_t hbuf = hs + hb * p.h_bytes;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (half + 2 * q < grans) {
+          if constexpr (kBwd) {
+            float dg[16], du[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float s = sigmoid(g[q][i]), act = g[q][i] * s;
+              du[i] = dh[q][i] * act;
+              dg[i] = dh[q][i] * u[q][i] * (s + act * (1.f - s));
+            }
+            store_granule(hbuf, row, half + 2 * q, dg);
+            store_granule(hbuf + kBlockBytes, row, half + 2 * q, du);
+          } else {
+            float h[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) h[i] = g[q][i] * sigmoid(g[q][i]) * u[q][i];
+            store_granule(hbuf, row, half + 2 * q, h);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bars.hfull[hb]);
+      if (j == 0 && it > 0) {  // the previous tile's output, while this one's products run
+        wait(&bars.yfull, it / p.nc - 1);
+        tc_fence_after();
+        store_output(p, yacc + quarter, tile - gridDim.x, out, half, row);
+        tc_fence_before();
+        mbar_arrive(&bars.yempty);
+      }
+      if (++j == p.nc) j = 0, tile += gridDim.x;
+    }
+    wait(&bars.yfull, mine - 1);
+    tc_fence_after();
+    store_output(p, yacc + quarter, tile - gridDim.x, out, half, row);
+  } else if (warp == 8) {
+    if (lane == 0) {
+      int slot = 0, round = 0;
+      auto acquire = [&](uint32_t fixed) {
+        if (p.resident) return ws + fixed;
+        wait(&bars.wfull[slot], round);
+        return ws + slot * kBlockBytes;
+      };
+      auto release = [&] {
+        if (p.resident) return;
+        tc_commit(&bars.wempty[slot]);
+        if (++slot == p.slots) slot = 0, ++round;
+      };
+      int j1 = 0, xb = 0, xround = 0;
+      auto first = [&](int it) {
+        const int b = p.nb == 2 ? it & 1 : 0;
+        const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
+        const uint32_t acc = tmem + b * kGCols;
+        if (j1 == 0) wait(&bars.xfull[xb], xround);
+        if (it >= p.nb) wait(&bars.gempty[b], p.nb == 2 ? (it >> 1) - 1 : it - 1);
+        tc_fence_after();
+        for (int c = 0; c < p.cd; ++c) {
+          const uint32_t w = acquire(wgu_offset(p, j1, c));
+          const int ks = min(4, p.kd - 4 * c);
+          for (int k = 0; k < ks; ++k)
+            tc_mma(acc, desc_k(x + c * kBlockBytes, k), desc_k(w, k), tc_idesc(128, false, false),
+                   c + k > 0);
+          release();
+        }
+        if constexpr (kBwd) {
+          for (int b8 = 0; b8 < wblocks; ++b8) {
+            const uint32_t w = acquire(wd_offset(p, j1, b8));
+            const int ks = min(8, p.ko - 8 * b8);
+            for (int k = 0; k < ks; ++k) {
+              const int kk = 8 * b8 + k;
+              tc_mma(acc + 128, desc_k(dy + (kk >> 2) * kBlockBytes, kk & 3),
+                     desc_mn(w, k, kBlockBytes), tc_idesc(64, false, true), kk > 0);
+            }
+            release();
+          }
+        }
+        tc_commit(&bars.gfull[b]);
+        if (++j1 == p.nc) {
+          tc_commit(&bars.xempty[xb]);
+          j1 = 0;
+          if (++xb == p.nx) xb = 0, ++xround;
+        }
+      };
+      int j = 0, t = 0;
+      first(0);
+      for (int it = 0; it < steps; ++it) {
+        if (it + 1 < steps) first(it + 1);
+        const int hb = p.nh == 2 ? it & 1 : 0;
+        wait(&bars.hfull[hb], p.nh == 2 ? it >> 1 : it);
+        if (j == 0 && t > 0) wait(&bars.yempty, t - 1);
+        tc_fence_after();
+        const uint32_t h = hs + hb * p.h_bytes;
+        const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
+        if constexpr (kBwd) {
+          // dG Wg + dU Wu: the blocks' columns are N, their rows K
+          const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
+          for (int c = 0; c < p.cd; c += wide) {
+            const uint32_t w = acquire(wgu_offset(p, j, c));
+            const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
+            for (int k = 0; k < ks; ++k)
+              tc_mma(yacc + 64 * c, desc_k(h, k), desc_mn(w, k, kBlockBytes), id, j + k > 0);
+            for (int k = 0; k < ks; ++k)
+              tc_mma(yacc + 64 * c, desc_k(h + kBlockBytes, k),
+                     desc_mn(w + 64 * 128, k, kBlockBytes), id, true);
+            release();
+          }
+        } else {
+          const int wide = p.resident ? wblocks : 1;
+          for (int b8 = 0; b8 < wblocks; b8 += wide) {
+            const uint32_t w = acquire(wd_offset(p, j, b8));
+            const uint32_t id = tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false);
+            for (int k = 0; k < ks; ++k)
+              tc_mma(yacc + 128 * b8, desc_k(h, k), desc_k(w, k), id, j + k > 0);
+            release();
+          }
+        }
+        tc_commit(&bars.hempty[hb]);
+        if (++j == p.nc) {
+          tc_commit(&bars.yfull);
+          j = 0, ++t;
+        }
+      }
+      tc_commit(&bars.done);
+      if (!mbar_wait_bounded(&bars.done, 0))
+        report_error(p.f.err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
+    }
+  } else if (warp == 9) {
+    if (lane == 0 && !p.resident) {
+      int slot = 0, round = 0;
+      auto put = [&](uint32_t offset, uint32_t bytes) {
+        if (round > 0) wait(&bars.wempty[slot], round - 1);
+        if (!wait.ok) return;  // after a wait that ran out, no copy may land in a slot in use
+        mbar_arrive_expect_tx(&bars.wfull[slot], bytes);
+        bulk_g2s(raw + (ws - smem_addr(raw)) + slot * kBlockBytes, p.packed + offset, bytes,
+                 &bars.wfull[slot]);
+        if (++slot == p.slots) slot = 0, ++round;
+      };
+      auto put_gu = [&](int j) {
+        for (int c = 0; c < p.cd; ++c) put(wgu_offset(p, j, c), kBlockBytes);
+      };
+      auto put_d = [&](int j) {
+        for (int b8 = 0; b8 < wblocks; ++b8)
+          put(wd_offset(p, j, b8), min(8, p.ko - 8 * b8) * 2048);
+      };
+      int j1 = 0, j = 0;
+      for (int it = -1; it < steps; ++it) {
+        if (it + 1 < steps) {
+          put_gu(j1);
+          if (kBwd) put_d(j1);
+          if (++j1 == p.nc) j1 = 0;
+        }
+        if (it >= 0) {
+          if (kBwd) {
+            put_gu(j);
+          } else {
+            put_d(j);
+          }
+          if (++j == p.nc) j = 0;
+        }
+        if (!wait.ok) break;
+      }
+      if (!wait.ok) {  // copies in flight land before the block leaves
+        for (int i = 0; i < p.slots; ++i) {
+          const int r = i < slot ? round : round - 1;
+          if (r >= 0) mbar_wait_bounded(&bars.wfull[i], r & 1);
+        }
+      }
+    }
+  } else {
+    const int tid = threadIdx.x - kEpi - 64;
+    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.f.x);
+    const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(p.f.dy);
+    int told = 0;  // tiles whose arrival has been signalled
+    auto tell = [&](int upto) {
+      fence_proxy_async_smem();
+      for (; told < upto; ++told) mbar_arrive(&bars.xfull[told % p.nx]);
+    };
+    for (int t = 0; t < mine; ++t) {
+      const int xb = t % p.nx;
+      if (t >= p.nx && !mbar_try_wait(&bars.xempty[xb], (t / p.nx - 1) & 1)) {
+        cp_async_wait<0>();  // nothing to issue: hand over what is on its way
+        tell(t);
+        wait(&bars.xempty[xb], t / p.nx - 1);
+      }
+      const int64_t r0 = (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile;
+      const uint32_t dst = xs + xb * p.tile_bytes;
+      load_tile(dst, x, p.f.x_stride, r0, p.f.n, p.f.d, p.kd, p.vec_x, tid);
+      if constexpr (kBwd)
+        load_tile(dst + p.cd * kBlockBytes, dy, p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, p.vec_dy, tid);
+      cp_async_commit();
+      cp_async_wait<1>();
+      tell(t);
+    }
+    cp_async_wait<0>();
+    tell(mine);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_free(tmem, p.tmem_cols);
+  }
+}
+
+uint32_t pow2_cols(uint32_t c) {
+  uint32_t p = 32;
+  while (p < c) p *= 2;
+  return p;
+}
+
+TcParams tc_params(const FfnParams& f) {
+  TcParams p{};
+  p.f = f;
+  p.kd = ceil_div(f.d, 16), p.ko = ceil_div(f.o, 16);
+  p.cd = ceil_div(f.d, 64), p.co = ceil_div(f.o, 64), p.nc = ceil_div(f.h, kChunk);
+  p.tiles = ceil_div<int64_t>(f.n, kTile);
+  p.w_bytes = static_cast<uint32_t>(p.nc) * (p.cd * kBlockBytes + p.ko * 2048);
+  p.vec_x = f.d % 8 == 0 && f.x_stride % 8 == 0 && aligned16(f.x);
+  p.vec_dy = f.o % 8 == 0 && f.dy_stride % 8 == 0 && aligned16(f.dy);
+  return p;
+}
+
+// Buffers of the rows kernel. Shared memory goes first to the weights (as a
+// whole where two row tiles and two hidden buffers fit beside them), then to
+// whatever keeps the most work in flight.
+void plan_rows(TcParams& p, bool bwd) {
+  p.tile_bytes = (p.cd + (bwd ? p.co : 0)) * kBlockBytes;
+  p.h_bytes = (bwd ? 2 : 1) * kBlockBytes;
+  const uint32_t out = bwd ? p.kd * 16 : p.ko * 16, g = bwd ? 192 : 128;
+  p.nb = 2 * g + out <= 512 ? 2 : 1;
+  p.tmem_cols = pow2_cols(p.nb * g + out);
+  const int64_t budget = kSmemBudget;
+  auto used = [&] { return static_cast<int64_t>(p.nx) * p.tile_bytes + p.nh * p.h_bytes; };
+  p.nx = 2, p.nh = 2, p.slots = 1;
+  p.resident = used() + p.w_bytes <= budget;
+  if (p.resident) {
+    p.nx = 3;
+    if (used() + p.w_bytes > budget) p.nx = 2;
+    return;
+  }
+  // The ring holds at least one chunk's blocks twice over before a second
+  // row tile or hidden buffer is bought with it.
+  const int per_chunk = p.cd + (p.ko + 7) / 8;
+  for (int more = 3; more >= 0; --more) {
+    p.nh = 1 + (more >> 1 & 1), p.nx = 1 + (more & 1);
+    p.slots = static_cast<int>(std::min<int64_t>(kMaxSlots, (budget - used()) / kBlockBytes));
+    if (p.slots >= std::min(2 * per_chunk, 6)) return;
+  }
+}
+
+uint32_t rows_smem(const TcParams& p) {
+  return p.nx * p.tile_bytes + p.nh * p.h_bytes +
+         (p.resident ? p.w_bytes : p.slots * kBlockBytes) + 1024;
+}
+
+template <bool kBwd>
+int launch_tc_rows(TcParams p, cudaStream_t s) {
+  plan_rows(p, kBwd);
+  const int out = kBwd ? p.f.d : p.f.o;
+  p.vec_y = out % 8 == 0 && aligned16(p.f.y);
+  if (!p.resident) {
+    uint8_t* packed = reinterpret_cast<uint8_t*>(p.f.scratch);
+    p.packed = packed;
+    ffn_pack_kernel<<<ceil_div<uint32_t>(p.w_bytes / 16, 256), 256, 0, s>>>(p, packed);
+    TGS_LAUNCH_CHECK();
+  }
+  const int smem = static_cast<int>(rows_smem(p));
+  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_rows_kernel<kBwd>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int grid = static_cast<int>(std::min<int64_t>(p.tiles, sm_count()));
+  ffn_tc_rows_kernel<kBwd><<<grid, kTcThreads, smem, s>>>(p);
+  TGS_LAUNCH_CHECK();
+  return TGS_OK;
+}
+
+}  // namespace
+
+int ffn_tc_forward(const FfnParams& f, cudaStream_t s) {
+  return launch_tc_rows<false>(tc_params(f), s);
+}
+
+int64_t ffn_tc_scratch_floats(int64_t n, int d, int h, int o, bool backward) {
+  FfnParams f{};
+  f.n = n, f.d = d, f.h = h, f.o = o;
+  TcParams p = tc_params(f);
+  plan_rows(p, backward);
+  return p.resident ? 0 : p.w_bytes / 4;
+}
+
+int ffn_tc_backward(const FfnParams& f, cudaStream_t s) {
+  return launch_tc_rows<true>(tc_params(f), s);
+}
+
+}  // namespace tgs
