@@ -34,13 +34,14 @@ constexpr int kMaxSlots = 12;  // weight ring
 constexpr int kSmemBudget = 227 * 1024 - 2048;  // less alignment and barriers
 
 struct TcParams {
+  CUtensorMap xmap, dymap;
   FfnParams f;
   const uint8_t* packed;  // laid-out weights (streaming)
   int64_t tiles;
   int cd, co, nc;  // operand blocks of D and O, chunks of H
   int kd, ko;      // 16-steps of D and O
   int nx, nh, nb, slots;
-  int resident, vec_x, vec_dy, vec_y;
+  int resident, tma_x, tma_dy, vec_y;
   uint32_t tile_bytes, h_bytes, w_bytes;
   uint32_t tmem_cols;
 };
@@ -155,21 +156,22 @@ __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint
   }
 }
 
-// Row tiles -> operand blocks: kd or ko 16-steps of columns, zeros beyond the
-// matrix.
+// A row tile -> operand blocks, by threads: for matrices that no tensor map
+// can describe. Thread -> one 16-byte unit of every eighth row of a block.
 __device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src, int64_t stride,
-                                          int64_t r0, int64_t n, int cols, int k16, bool vec,
-                                          int tid) {
-  const int units = 2 * k16;
-  for (int e = tid; e < kTile * units; e += kLoad) {
-    const int row = e / units, unit = e - row * units;
-    const bool on = r0 + row < n && unit * 8 < cols;
-    const uint32_t at = dst + (unit >> 3) * kBlockBytes + unit_offset(row, unit & 7);
-    const int64_t from = on ? (r0 + row) * stride + unit * 8 : 0;
-    if (vec) {
-      cp_async16(at, src + from, on);
-    } else {
-      st_shared16(at, on ? load_unit(src, from, cols - unit * 8, false) : make_uint4(0, 0, 0, 0));
+                                          int64_t r0, int64_t n, int cols, int k16, int tid) {
+  static_assert(kLoad == 64, "eight rows of eight units per pass");
+  const int unit = tid & 7;
+  for (int c = 0; 8 * c < 2 * k16; ++c) {
+    if (unit >= 2 * k16 - 8 * c) continue;
+    const int col = c * kBlockCols + unit * 8;
+    uint32_t at = dst + c * kBlockBytes + unit_offset(tid >> 3, unit);
+    const __nv_bfloat16* from = src + (r0 + (tid >> 3)) * stride + col;
+    int64_t left = n - r0 - (tid >> 3);
+#pragma unroll 2
+    for (int i = 0; i < kTile / 8; ++i) {
+      st_shared16(at, left > 0 ? load_unit(from, 0, cols - col, false) : make_uint4(0, 0, 0, 0));
+      at += 1024, from += 8 * stride, left -= 8;
     }
   }
 }
@@ -207,7 +209,7 @@ __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, in
 
 // --- rows: Y, or dX --------------------------------------------------------------
 template <bool kBwd>
-__global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const TcParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid_constant__ TcParams p) {
   extern __shared__ uint8_t raw[];
   __shared__ TcBars bars;
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -454,29 +456,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const TcPara
     const int tid = threadIdx.x - kEpi - 64;
     const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.f.x);
     const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(p.f.dy);
-    int told = 0;  // tiles whose arrival has been signalled
-    auto tell = [&](int upto) {
-      fence_proxy_async_smem();
-      for (; told < upto; ++told) mbar_arrive(&bars.xfull[told % p.nx]);
-    };
+    int xb = 0, round = 0;
     for (int t = 0; t < mine; ++t) {
-      const int xb = t % p.nx;
-      if (t >= p.nx && !mbar_try_wait(&bars.xempty[xb], (t / p.nx - 1) & 1)) {
-        cp_async_wait<0>();  // nothing to issue: hand over what is on its way
-        tell(t);
-        wait(&bars.xempty[xb], t / p.nx - 1);
-      }
+      if (round > 0) wait(&bars.xempty[xb], round - 1);
       const int64_t r0 = (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile;
       const uint32_t dst = xs + xb * p.tile_bytes;
-      load_tile(dst, x, p.f.x_stride, r0, p.f.n, p.f.d, p.kd, p.vec_x, tid);
-      if constexpr (kBwd)
-        load_tile(dst + p.cd * kBlockBytes, dy, p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, p.vec_dy, tid);
-      cp_async_commit();
-      cp_async_wait<1>();
-      tell(t);
+      const bool both = kBwd && !p.tma_dy;
+      if (!p.tma_x) load_tile(dst, x, p.f.x_stride, r0, p.f.n, p.f.d, p.kd, tid);
+      if (both)
+        load_tile(dst + p.cd * kBlockBytes, dy, p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, tid);
+      if (!p.tma_x || both) fence_proxy_async_smem();
+      if (tid > 0) {
+        mbar_arrive(&bars.xfull[xb]);
+      } else if (wait.ok) {
+        const int xblocks = p.tma_x ? p.cd : 0, yblocks = kBwd && p.tma_dy ? p.co : 0;
+        mbar_arrive_expect_tx(&bars.xfull[xb], (xblocks + yblocks) * kBlockBytes);
+        for (int c = 0; c < xblocks; ++c)
+          tma_load_2d(dst + c * kBlockBytes, &p.xmap, c * kBlockCols, static_cast<int>(r0),
+                      &bars.xfull[xb]);
+        for (int c = 0; c < yblocks; ++c)
+          tma_load_2d(dst + (p.cd + c) * kBlockBytes, &p.dymap, c * kBlockCols,
+                      static_cast<int>(r0), &bars.xfull[xb]);
+      }
+      if (++xb == p.nx) xb = 0, ++round;
     }
-    cp_async_wait<0>();
-    tell(mine);
+    if (tid == 0 && !wait.ok) {  // copies in flight land before the block leaves
+      for (int i = 0; i < p.nx; ++i) {
+        const int r = i < xb ? round : round - 1;
+        if (r >= 0) mbar_wait_bounded(&bars.xfull[i], r & 1);
+      }
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -500,9 +509,18 @@ TcParams tc_params(const FfnParams& f) {
   p.cd = ceil_div(f.d, 64), p.co = ceil_div(f.o, 64), p.nc = ceil_div(f.h, kChunk);
   p.tiles = ceil_div<int64_t>(f.n, kTile);
   p.w_bytes = static_cast<uint32_t>(p.nc) * (p.cd * kBlockBytes + p.ko * 2048);
-  p.vec_x = f.d % 8 == 0 && f.x_stride % 8 == 0 && aligned16(f.x);
-  p.vec_dy = f.o % 8 == 0 && f.dy_stride % 8 == 0 && aligned16(f.dy);
   return p;
+}
+
+// Tensor maps for the matrices that have one; threads load the others.
+int make_maps(TcParams& p, bool bwd) {
+  const FfnParams& f = p.f;
+  p.tma_x = f.x_stride % 8 == 0 && aligned16(f.x);
+  p.tma_dy = bwd && f.dy_stride % 8 == 0 && aligned16(f.dy);
+  if (p.tma_x) {
+    if (int rc = make_row_map(&p.xmap, f.x, f.n, f.d, f.x_stride)) return rc;
+  }
+  return p.tma_dy ? make_row_map(&p.dymap, f.dy, f.n, f.o, f.dy_stride) : TGS_OK;
 }
 
 // Buffers of the rows kernel. Shared memory goes first to the weights (as a
@@ -541,6 +559,7 @@ uint32_t rows_smem(const TcParams& p) {
 template <bool kBwd>
 int launch_tc_rows(TcParams p, cudaStream_t s) {
   plan_rows(p, kBwd);
+  if (int rc = make_maps(p, kBwd)) return rc;
   const int out = kBwd ? p.f.d : p.f.o;
   p.vec_y = out % 8 == 0 && aligned16(p.f.y);
   if (!p.resident) {
@@ -559,6 +578,30 @@ int launch_tc_rows(TcParams p, cudaStream_t s) {
 }
 
 }  // namespace
+
+int make_row_map(CUtensorMap* map, const void* base, int64_t rows, int cols, int64_t stride) {
+  static decltype(&cuTensorMapEncodeTiled) encode = nullptr;
+  if (encode == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    TGS_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
+    TGS_CHECK_ARG(fn != nullptr, "cuTensorMapEncodeTiled is missing from the driver");
+    encode = reinterpret_cast<decltype(encode)>(fn);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  const cuuint32_t box[2] = {kBlockCols, 128}, steps[2] = {1, 1};
+  const CUresult rc =
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+             steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d): %lld rows x %d, stride %lld", static_cast<int>(rc),
+              static_cast<long long>(rows), cols, static_cast<long long>(stride));
+    return TGS_ERR_CUDA;
+  }
+  return TGS_OK;
+}
 
 int ffn_tc_forward(const FfnParams& f, cudaStream_t s) {
   return launch_tc_rows<false>(tc_params(f), s);

@@ -7,6 +7,8 @@
 // ("K-major"), or with its columns as M or N and its rows as K ("MN-major").
 #pragma once
 
+#include <cuda.h>
+
 #include "tgs_common.cuh"
 
 namespace tgs {
@@ -115,18 +117,20 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
                : "memory");
 }
 
-// 16 bytes global -> shared, or zeros where !on; completes with the group.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0)
-               : "memory");
+// One box of a 2-D tensor map -> shared memory, completion counted on `bar`.
+// `col` x the element size is a multiple of 16 bytes.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int col, int row,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(col), "r"(row), "r"(smem_addr(bar))
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+
+// Map of a row-major bf16 matrix for boxes of 128 rows x 64 columns in the
+// operand layout, zeros outside the matrix. The base is 16-byte aligned and
+// the row stride a multiple of 8 elements. Returns a TGS_ status.
+int make_row_map(CUtensorMap* map, const void* base, int64_t rows, int cols, int64_t stride);
 
 }  // namespace tgs
