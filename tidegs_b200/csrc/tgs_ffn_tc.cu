@@ -8,8 +8,10 @@
 // products add that chunk's share to the output tile's accumulators (Y, or
 // dX). The roles are warps of their own joined by mbarriers, so loads,
 // products and the activation of different chunks run at once:
-//   warps 0-7   activation, output        warp 8   issues matrix instructions
-//   warp  9     weight blocks (bulk copies)  warps 10-11   row tiles
+//   warps 0-7    activation, output: two groups of four take turns by chunk
+//   warp  8      issues the matrix instructions
+//   warp  9      weight blocks (bulk copies)
+//   warps 10-11  row tiles (tensor-map copies)
 // The same block of weights serves both products: as K-major operand of one
 // and as MN-major operand of the other.
 //
@@ -49,7 +51,7 @@ struct TcParams {
 struct TcBars {
   uint64_t xfull[kMaxTiles], xempty[kMaxTiles];
   uint64_t gfull[2], gempty[2], hfull[2], hempty[2];
-  uint64_t yfull, yempty, done;
+  uint64_t yfull[2], yempty, done;
   uint64_t wfull[kMaxSlots], wempty[kMaxSlots];
   uint32_t tmem;
 };
@@ -127,6 +129,13 @@ struct Waits {
   }
 };
 
+// One arrival for the warp, after all of its lanes have come here (an arrival
+// per thread takes as long as the activation: they are counted one by one).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
 // --- activation --------------------------------------------------------------------
 __device__ __forceinline__ float fast_exp2(float x) {
   float r;
@@ -177,10 +186,10 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src
 }
 
 __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, int64_t tile,
-                                             int out, int half, int lane_row) {
+                                             int out, int lane_row) {
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.f.y);
   const int64_t row = tile * kTile + lane_row;
-  for (int c = half * 16; c < out; c += 32) {
+  for (int c = 0; c < out; c += 16) {
     float v[16];
     tmem_ld16(acc + c, v);
     tmem_wait_ld(v);
@@ -216,7 +225,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   const uint32_t xs = base;                             // nx tiles: X blocks, then dY blocks
   const uint32_t hs = xs + p.nx * p.tile_bytes;         // nh hidden buffers
   const uint32_t ws = hs + p.nh * p.h_bytes;            // weights, or the ring
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // from lane 0, so that the compiler sees the roles' branches as uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int mine = static_cast<int>((p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
   const int steps = mine * p.nc;  // n <= 2^31 and H <= 4096: below 2^30 of them
   const int wblocks = (p.ko + 7) / 8;  // blocks of Wd per chunk
@@ -226,12 +236,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   if (warp == 8) {
     tmem_alloc(&bars.tmem, p.tmem_cols);
     if (lane == 0) {
-      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], kLoad), mbar_init(&bars.xempty[i], 1);
+      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], kLoad / 32), mbar_init(&bars.xempty[i], 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], kEpi);
-        mbar_init(&bars.hfull[i], kEpi), mbar_init(&bars.hempty[i], 1);
+        mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], 4);
+        mbar_init(&bars.hfull[i], 4), mbar_init(&bars.hempty[i], 1);
+        mbar_init(&bars.yfull[i], 1);
       }
-      mbar_init(&bars.yfull, 1), mbar_init(&bars.yempty, kEpi), mbar_init(&bars.done, 1);
+      mbar_init(&bars.yempty, 4), mbar_init(&bars.done, 1);
       for (int i = 0; i < kMaxSlots; ++i) mbar_init(&bars.wfull[i], 1), mbar_init(&bars.wempty[i], 1);
       fence_mbar_init();
     }
@@ -250,166 +261,151 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   const uint32_t tmem = bars.tmem;
   const uint32_t yacc = tmem + p.nb * kGCols;
 
+  // Step `it` (tile it / nc, chunk it % nc) signals on the barriers of its
+  // parity, whether or not there are two buffers: each side then meets every
+  // phase of a barrier in turn.
   if (warp < 8) {
-    // Activation: this thread's row of the tile, 16-column granules half,
-    // half + 2 of the chunk.
+    // Activation: group warp / 4 takes the steps of its parity; this thread's
+    // row of the tile.
     const uint32_t row = (warp & 3) * 32 + lane;
-    const int half = warp >> 2;
+    const int group = warp >> 2;
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane 32 (warp % 4)
-    int j = 0;
-    int64_t tile = blockIdx.x;
+    int j = group;
     const int out = kBwd ? p.f.d : p.f.o;
-    for (int it = 0; it < steps; ++it) {
-      const int b = p.nb == 2 ? it & 1 : 0, hb = p.nh == 2 ? it & 1 : 0;
-      wait(&bars.gfull[b], p.nb == 2 ? it >> 1 : it);
+    auto output = [&](int t) {
+      wait(&bars.yfull[t & 1], t >> 1);
       tc_fence_after();
-      const uint32_t acc = tmem + b * kGCols + quarter;
-      const int grans = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
-      float g[2][16], u[2][16], dh[2][16];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if (half + 2 * q < grans) {
-          tmem_ld16(acc + (half + 2 * q) * 16, g[q]);
-          tmem_ld16(acc + 64 + (half + 2 * q) * 16, u[q]);
-          if constexpr (kBwd) tmem_ld16(acc + 128 + (half + 2 * q) * 16, dh[q]);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        tmem_wait_ld(g[q]);
-        tmem_wait_ld(u[q]);
-        if constexpr (kBwd) tmem_wait_ld(dh[q]);
-      }
+      store_output(p, yacc + quarter, blockIdx.x + static_cast<int64_t>(t) * gridDim.x, out, row);
       tc_fence_before();
-      mbar_arrive(&bars.gempty[b]);
-      if (it >= p.nh) wait(&bars.hempty[hb], p.nh == 2 ? (it >> 1) - 1 : it - 1);
-      const uint32_t hbuf = hs + hb * p.h_bytes;
+      warp_arrive(&bars.yempty, lane);
+    };
+    for (int it = group, t = 0; it < steps; it += 2, j += 2) {
+      while (j >= p.nc) j -= p.nc, ++t;
+      wait(&bars.gfull[group], it >> 1);
+      tc_fence_after();
+      const uint32_t acc = tmem + (p.nb == 2 ? group : 0) * kGCols + quarter;
+      const uint32_t hbuf = hs + (p.nh == 2 ? group : 0) * p.h_bytes;
+      const int grans = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
+      const int before = it - p.nh;  // the step that last used the hidden buffer
+      if (before >= 0) wait(&bars.hempty[before & 1], before >> 1);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if (half + 2 * q < grans) {
+      for (int q = 0; q < 4; ++q) {
+        if (q < grans) {
+          float g[16], u[16], dh[16];
+          tmem_ld16(acc + q * 16, g);
+          tmem_ld16(acc + 64 + q * 16, u);
+          if constexpr (kBwd) tmem_ld16(acc + 128 + q * 16, dh);
+          tmem_wait_ld(g);
+          tmem_wait_ld(u);
           if constexpr (kBwd) {
-            float dg[16], du[16];
+            tmem_wait_ld(dh);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float s = sigmoid(g[q][i]), act = g[q][i] * s;
-              du[i] = dh[q][i] * act;
-              dg[i] = dh[q][i] * u[q][i] * (s + act * (1.f - s));
+              const float s = sigmoid(g[i]), act = g[i] * s, d = dh[i];
+              dh[i] = d * act;                               // dU
+              g[i] = d * u[i] * (s + act * (1.f - s));       // dG
             }
-            store_granule(hbuf, row, half + 2 * q, dg);
-            store_granule(hbuf + kBlockBytes, row, half + 2 * q, du);
+            store_granule(hbuf, row, q, g);
+            store_granule(hbuf + kBlockBytes, row, q, dh);
           } else {
-            float h[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) h[i] = g[q][i] * sigmoid(g[q][i]) * u[q][i];
-            store_granule(hbuf, row, half + 2 * q, h);
+            for (int i = 0; i < 16; ++i) g[i] = g[i] * sigmoid(g[i]) * u[i];
+            store_granule(hbuf, row, q, g);
           }
         }
       }
+      tc_fence_before();
       fence_proxy_async_smem();
-      mbar_arrive(&bars.hfull[hb]);
-      if (j == 0 && it > 0) {  // the previous tile's output, while this one's products run
-        wait(&bars.yfull, it / p.nc - 1);
-        tc_fence_after();
-        store_output(p, yacc + quarter, tile - gridDim.x, out, half, row);
-        tc_fence_before();
-        mbar_arrive(&bars.yempty);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars.gempty[group]);
+        mbar_arrive(&bars.hfull[group]);
       }
-      if (++j == p.nc) j = 0, tile += gridDim.x;
+      if (j == 0 && it > 0) output(t - 1);  // while this tile's products run
     }
-    wait(&bars.yfull, mine - 1);
-    tc_fence_after();
-    store_output(p, yacc + quarter, tile - gridDim.x, out, half, row);
+    if (group == (steps & 1)) output(mine - 1);
   } else if (warp == 8) {
-    if (lane == 0) {
-      int slot = 0, round = 0;
-      auto acquire = [&](uint32_t fixed) {
-        if (p.resident) return ws + fixed;
-        wait(&bars.wfull[slot], round);
-        return ws + slot * kBlockBytes;
-      };
-      auto release = [&] {
-        if (p.resident) return;
-        tc_commit(&bars.wempty[slot]);
-        if (++slot == p.slots) slot = 0, ++round;
-      };
-      int j1 = 0, xb = 0, xround = 0;
-      auto first = [&](int it) {
-        const int b = p.nb == 2 ? it & 1 : 0;
-        const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
-        const uint32_t acc = tmem + b * kGCols;
-        if (j1 == 0) wait(&bars.xfull[xb], xround);
-        if (it >= p.nb) wait(&bars.gempty[b], p.nb == 2 ? (it >> 1) - 1 : it - 1);
-        tc_fence_after();
-        for (int c = 0; c < p.cd; ++c) {
-          const uint32_t w = acquire(wgu_offset(p, j1, c));
-          const int ks = min(4, p.kd - 4 * c);
-          for (int k = 0; k < ks; ++k)
-            tc_mma(acc, desc_k(x + c * kBlockBytes, k), desc_k(w, k), tc_idesc(128, false, false),
-                   c + k > 0);
+    int slot = 0, round = 0;
+    auto acquire = [&](uint32_t fixed) {
+      if (p.resident) return ws + fixed;
+      wait(&bars.wfull[slot], round);
+      return ws + slot * kBlockBytes;
+    };
+    auto release = [&] {
+      if (p.resident) return;
+      tc_commit(&bars.wempty[slot]);
+      if (++slot == p.slots) slot = 0, ++round;
+    };
+    int j1 = 0, xb = 0, xround = 0;
+    auto first = [&](int it) {
+      const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
+      const uint32_t acc = tmem + (p.nb == 2 ? it & 1 : 0) * kGCols;
+      if (j1 == 0) wait(&bars.xfull[xb], xround);
+      const int before = it - p.nb;
+      if (before >= 0) wait(&bars.gempty[before & 1], before >> 1);
+      tc_fence_after();
+      for (int c = 0; c < p.cd; ++c) {
+        const uint32_t w = acquire(wgu_offset(p, j1, c));
+        tc_mma_steps<4>(acc, desc_k(x + c * kBlockBytes), kStepK, desc_k(w), kStepK,
+                        tc_idesc(128, false, false), p.kd - 4 * c, c > 0);
+        release();
+      }
+      if constexpr (kBwd) {
+        for (int b8 = 0; b8 < wblocks; ++b8) {
+          const uint32_t w = acquire(wd_offset(p, j1, b8));
+          for (int c = 0; c < 2 && 2 * b8 + c < p.co; ++c)
+            tc_mma_steps<4>(acc + 128, desc_k(dy + (2 * b8 + c) * kBlockBytes), kStepK,
+                            desc_mn(w + c * 64 * 128, kBlockBytes), kStepMn,
+                            tc_idesc(64, false, true), p.ko - 8 * b8 - 4 * c, b8 + c > 0);
           release();
         }
-        if constexpr (kBwd) {
-          for (int b8 = 0; b8 < wblocks; ++b8) {
-            const uint32_t w = acquire(wd_offset(p, j1, b8));
-            const int ks = min(8, p.ko - 8 * b8);
-            for (int k = 0; k < ks; ++k) {
-              const int kk = 8 * b8 + k;
-              tc_mma(acc + 128, desc_k(dy + (kk >> 2) * kBlockBytes, kk & 3),
-                     desc_mn(w, k, kBlockBytes), tc_idesc(64, false, true), kk > 0);
-            }
-            release();
-          }
+      }
+      tc_commit(&bars.gfull[it & 1]);
+      if (++j1 == p.nc) {
+        tc_commit(&bars.xempty[xb]);
+        j1 = 0;
+        if (++xb == p.nx) xb = 0, ++xround;
+      }
+    };
+    int j = 0, t = 0;
+    first(0);
+    for (int it = 0; it < steps; ++it) {
+      if (it + 1 < steps) first(it + 1);
+      wait(&bars.hfull[it & 1], it >> 1);
+      if (j == 0 && t > 0) wait(&bars.yempty, t - 1);
+      tc_fence_after();
+      const uint32_t h = hs + (p.nh == 2 ? it & 1 : 0) * p.h_bytes;
+      const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
+      if constexpr (kBwd) {
+        // dG Wg + dU Wu: the blocks' columns are N, their rows K
+        const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
+        for (int c = 0; c < p.cd; c += wide) {
+          const uint32_t w = acquire(wgu_offset(p, j, c));
+          const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
+          tc_mma_steps<4>(yacc + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
+                          ks, j > 0);
+          tc_mma_steps<4>(yacc + 64 * c, desc_k(h + kBlockBytes), kStepK,
+                          desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
+          release();
         }
-        tc_commit(&bars.gfull[b]);
-        if (++j1 == p.nc) {
-          tc_commit(&bars.xempty[xb]);
-          j1 = 0;
-          if (++xb == p.nx) xb = 0, ++xround;
-        }
-      };
-      int j = 0, t = 0;
-      first(0);
-      for (int it = 0; it < steps; ++it) {
-        if (it + 1 < steps) first(it + 1);
-        const int hb = p.nh == 2 ? it & 1 : 0;
-        wait(&bars.hfull[hb], p.nh == 2 ? it >> 1 : it);
-        if (j == 0 && t > 0) wait(&bars.yempty, t - 1);
-        tc_fence_after();
-        const uint32_t h = hs + hb * p.h_bytes;
-        const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
-        if constexpr (kBwd) {
-          // dG Wg + dU Wu: the blocks' columns are N, their rows K
-          const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
-          for (int c = 0; c < p.cd; c += wide) {
-            const uint32_t w = acquire(wgu_offset(p, j, c));
-            const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
-            for (int k = 0; k < ks; ++k)
-              tc_mma(yacc + 64 * c, desc_k(h, k), desc_mn(w, k, kBlockBytes), id, j + k > 0);
-            for (int k = 0; k < ks; ++k)
-              tc_mma(yacc + 64 * c, desc_k(h + kBlockBytes, k),
-                     desc_mn(w + 64 * 128, k, kBlockBytes), id, true);
-            release();
-          }
-        } else {
-          const int wide = p.resident ? wblocks : 1;
-          for (int b8 = 0; b8 < wblocks; b8 += wide) {
-            const uint32_t w = acquire(wd_offset(p, j, b8));
-            const uint32_t id = tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false);
-            for (int k = 0; k < ks; ++k)
-              tc_mma(yacc + 128 * b8, desc_k(h, k), desc_k(w, k), id, j + k > 0);
-            release();
-          }
-        }
-        tc_commit(&bars.hempty[hb]);
-        if (++j == p.nc) {
-          tc_commit(&bars.yfull);
-          j = 0, ++t;
+      } else {
+        const int wide = p.resident ? wblocks : 1;
+        for (int b8 = 0; b8 < wblocks; b8 += wide) {
+          const uint32_t w = acquire(wd_offset(p, j, b8));
+          tc_mma_steps<4>(yacc + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
+                          tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks, j > 0);
+          release();
         }
       }
-      tc_commit(&bars.done);
-      if (!mbar_wait_bounded(&bars.done, 0))
-        report_error(p.f.err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
+      tc_commit(&bars.hempty[it & 1]);
+      if (++j == p.nc) {
+        tc_commit(&bars.yfull[t & 1]);
+        j = 0, ++t;
+      }
     }
+    tc_commit(&bars.done);
+    if (!mbar_wait_bounded(&bars.done, 0))
+      report_error(p.f.err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
   } else if (warp == 9) {
     if (lane == 0 && !p.resident) {
       int slot = 0, round = 0;
@@ -466,9 +462,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       if (both)
         load_tile(dst + p.cd * kBlockBytes, dy, p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, tid);
       if (!p.tma_x || both) fence_proxy_async_smem();
-      if (tid > 0) {
-        mbar_arrive(&bars.xfull[xb]);
-      } else if (wait.ok) {
+      if (warp == 11) {
+        warp_arrive(&bars.xfull[xb], lane);
+      } else if (__syncwarp(), lane == 0 && wait.ok) {
         const int xblocks = p.tma_x ? p.cd : 0, yblocks = kBwd && p.tma_dy ? p.co : 0;
         mbar_arrive_expect_tx(&bars.xfull[xb], (xblocks + yblocks) * kBlockBytes);
         for (int c = 0; c < xblocks; ++c)

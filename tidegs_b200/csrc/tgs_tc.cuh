@@ -21,23 +21,23 @@ __host__ __device__ __forceinline__ uint32_t unit_offset(uint32_t row, uint32_t 
   return row * 128 + ((unit ^ (row & 7)) << 4);
 }
 
-// Shared-memory matrix descriptor: address / 16, leading and stride offsets /
-// 16, descriptor version 1 (bits 46-47), 128-byte swizzle (bits 61-63 = 2).
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead_bytes) {
-  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) |
-         (static_cast<uint64_t>(lead_bytes >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
+// Shared-memory matrix descriptors, the low word (address / 16, leading
+// offset / 16 from bit 16) apart from the high one, which is the same for all:
+// stride offset 1024 / 16, descriptor version 1 (bits 46-47), 128-byte swizzle
+// (bits 61-63 = 2). Steps of K are additions to the low word.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 
 // K-major: 16 columns of K per instruction, 32 bytes along the row.
-__device__ __forceinline__ uint64_t desc_k(uint32_t block, int k16) {
-  return tc_desc(block + k16 * 32, 16);
+constexpr uint32_t kStepK = 32 >> 4;
+__device__ __forceinline__ uint32_t desc_k(uint32_t block) {
+  return ((block & 0x3FFFF) >> 4) | (1u << 16);
 }
 
 // MN-major: 16 rows of K per instruction, 2048 bytes; 64 columns of M or N
 // per block, the next 64 in the block `lead` bytes on.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t block, int k16, uint32_t lead) {
-  return tc_desc(block + k16 * 2048, lead);
+constexpr uint32_t kStepMn = 2048 >> 4;
+__device__ __forceinline__ uint32_t desc_mn(uint32_t block, uint32_t lead) {
+  return ((block & 0x3FFFF) >> 4) | ((lead >> 4) << 16);
 }
 
 // Instruction descriptor: fp32 accumulators, bf16 operands, M = 128.
@@ -46,23 +46,55 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool a_mn, bool b_mn) {
          (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void tc_mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc,
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(on));
+  return on != 0;
+}
+
+__device__ __forceinline__ void tc_mma(uint32_t acc, uint32_t a, uint32_t b, uint32_t idesc,
                                        bool accumulate) {
   asm volatile(
       "{\n"
       ".reg .pred p;\n"
+      ".reg .b64 da, db;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "mov.b64 da, {%1, %5};\n"
+      "mov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
       "}\n" ::"r"(acc),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(kDescHigh)
       : "memory");
+}
+
+// kMost or fewer (`steps`) instructions along K, issued by one lane; the
+// whole warp comes here.
+template <int kMost>
+__device__ __forceinline__ void tc_mma_steps(uint32_t acc, uint32_t a, uint32_t a_step, uint32_t b,
+                                             uint32_t b_step, uint32_t idesc, int steps,
+                                             bool accumulate) {
+  if (elect_one()) {
+#pragma unroll
+    for (int k = 0; k < kMost; ++k)
+      if (k < steps) tc_mma(acc, a + k * a_step, b + k * b_step, idesc, accumulate || k > 0);
+  }
+  __syncwarp();
 }
 
 // Arrives on `bar` when every matrix instruction issued so far has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
-               : "memory");
+  if (elect_one())
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                     smem_addr(bar))
+                 : "memory");
+  __syncwarp();
 }
 
 __device__ __forceinline__ void tc_fence_before() {
