@@ -9,9 +9,11 @@
 // dX). The roles are warps of their own joined by mbarriers, so loads,
 // products and the activation of different chunks run at once:
 //   warps 0-7    activation, output: two groups of four take turns by chunk
-//   warp  8      issues the matrix instructions
-//   warp  9      weight blocks (bulk copies)
-//   warps 10-11  row tiles (tensor-map copies)
+//   warps 8, 9   issue the first and the second products (a warp each: the
+//                next chunk's first products do not wait behind the output)
+//   warp  10     weight blocks (bulk copies)
+//   warp  11     row tiles by tensor-map copies
+//   warps 12-15  row tiles that no tensor map describes
 // The same block of weights serves both products: as K-major operand of one
 // and as MN-major operand of the other.
 //
@@ -27,8 +29,8 @@ namespace tgs {
 namespace {
 
 constexpr int kEpi = 256;      // activation threads
-constexpr int kLoad = 64;      // row-tile threads
-constexpr int kTcThreads = kEpi + 64 + kLoad;
+constexpr int kLoad = 128;     // threads for rows that no tensor map describes
+constexpr int kTcThreads = kEpi + 128 + kLoad;
 constexpr int kTile = 128;     // rows
 constexpr int kChunk = 64;     // hidden values
 constexpr int kMaxTiles = 3;   // row-tile buffers
@@ -122,7 +124,7 @@ struct Waits {
   int32_t* err;
   bool ok = true;
   __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t phase) {
-    if (ok && !mbar_wait_bounded(bar, phase & 1)) {
+    if (ok && !tc_wait(bar, phase & 1)) {
       ok = false;
       report_error(err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
     }
@@ -151,6 +153,27 @@ __device__ __forceinline__ float sigmoid(float g) {
   return fast_rcp(1.f + fast_exp2(g * -1.4426950408889634f));
 }
 
+// s[i] = 1 / (1 + exp(-g[i])). The special-function unit (16 results a cycle
+// and SM) bounds the activation, so two values share a reciprocal, 1 / a =
+// b / (a b): 1.5 of its operations a value instead of 2. Where a product
+// leaves the range (g below -43, infinity, NaN) the values get one each.
+__device__ __forceinline__ void sigmoid16(const float (&g)[16], float (&s)[16]) {
+  bool wide = false;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const float a = 1.f + fast_exp2(g[i] * -1.4426950408889634f);
+    const float b = 1.f + fast_exp2(g[i + 1] * -1.4426950408889634f);
+    const float ab = a * b;
+    wide |= !(ab < 0x1p126f);
+    const float r = fast_rcp(ab);
+    s[i] = r * b, s[i + 1] = r * a;
+  }
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = sigmoid(g[i]);
+  }
+}
+
 // Writes 16 values as bf16 into units 2 g16 and 2 g16 + 1 of a block's row.
 __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint32_t g16,
                                               const float (&v)[16]) {
@@ -166,10 +189,10 @@ __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint
 }
 
 // A row tile -> operand blocks, by threads: for matrices that no tensor map
-// can describe. Thread -> one 16-byte unit of every eighth row of a block.
+// can describe. Thread -> one 16-byte unit of every 16th row of a block.
 __device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src, int64_t stride,
                                           int64_t r0, int64_t n, int cols, int k16, int tid) {
-  static_assert(kLoad == 64, "eight rows of eight units per pass");
+  static_assert(kLoad == 128, "sixteen rows of eight units per pass");
   const int unit = tid & 7;
   for (int c = 0; 8 * c < 2 * k16; ++c) {
     if (unit >= 2 * k16 - 8 * c) continue;
@@ -178,18 +201,18 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src
     const __nv_bfloat16* from = src + (r0 + (tid >> 3)) * stride + col;
     int64_t left = n - r0 - (tid >> 3);
 #pragma unroll 2
-    for (int i = 0; i < kTile / 8; ++i) {
+    for (int i = 0; i < kTile / 16; ++i) {
       st_shared16(at, left > 0 ? load_unit(from, 0, cols - col, false) : make_uint4(0, 0, 0, 0));
-      at += 1024, from += 8 * stride, left -= 8;
+      at += 2048, from += 16 * stride, left -= 16;
     }
   }
 }
 
 __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, int64_t tile,
-                                             int out, int lane_row) {
+                                             int out, int lane_row, int from, int step) {
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.f.y);
   const int64_t row = tile * kTile + lane_row;
-  for (int c = 0; c < out; c += 16) {
+  for (int c = from; c < out; c += step) {
     float v[16];
     tmem_ld16(acc + c, v);
     tmem_wait_ld(v);
@@ -236,13 +259,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   if (warp == 8) {
     tmem_alloc(&bars.tmem, p.tmem_cols);
     if (lane == 0) {
-      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], kLoad / 32), mbar_init(&bars.xempty[i], 1);
+      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], 1 + kLoad / 32), mbar_init(&bars.xempty[i], 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], 4);
         mbar_init(&bars.hfull[i], 4), mbar_init(&bars.hempty[i], 1);
         mbar_init(&bars.yfull[i], 1);
       }
-      mbar_init(&bars.yempty, 4), mbar_init(&bars.done, 1);
+      mbar_init(&bars.yempty, p.nc > 1 && p.nh == 2 ? 8 : 4), mbar_init(&bars.done, 2);
       for (int i = 0; i < kMaxSlots; ++i) mbar_init(&bars.wfull[i], 1), mbar_init(&bars.wempty[i], 1);
       fence_mbar_init();
     }
@@ -272,13 +295,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane 32 (warp % 4)
     int j = group;
     const int out = kBwd ? p.f.d : p.f.o;
+    // A tile's output is stored by both groups, every second granule each,
+    // after their first step in the next tile; of one chunk to a tile, or with
+    // one hidden buffer (where a group's step waits for products that wait for
+    // that output), by the group that has the next tile's first step.
+    const int share = p.nc > 1 && p.nh == 2 ? 2 : 1;
     auto output = [&](int t) {
       wait(&bars.yfull[t & 1], t >> 1);
       tc_fence_after();
-      store_output(p, yacc + quarter, blockIdx.x + static_cast<int64_t>(t) * gridDim.x, out, row);
+      store_output(p, yacc + quarter, blockIdx.x + static_cast<int64_t>(t) * gridDim.x, out, row,
+                   share == 2 ? group * 16 : 0, share * 16);
       tc_fence_before();
       warp_arrive(&bars.yempty, lane);
     };
+    int told = 0;  // tiles whose output this group has stored (share 2)
     for (int it = group, t = 0; it < steps; it += 2, j += 2) {
       while (j >= p.nc) j -= p.nc, ++t;
       wait(&bars.gfull[group], it >> 1);
@@ -288,125 +318,150 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       const int grans = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
       const int before = it - p.nh;  // the step that last used the hidden buffer
       if (before >= 0) wait(&bars.hempty[before & 1], before >> 1);
+      // Granules of 16 columns; the next one is on its way from tensor memory
+      // while one is computed.
+      constexpr int kParts = kBwd ? 3 : 2;  // G, U, dH
+      float v[2][kParts][16];
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) tmem_ld16(acc + 64 * k, v[0][k]);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (q < grans) {
-          float g[16], u[16], dh[16];
-          tmem_ld16(acc + q * 16, g);
-          tmem_ld16(acc + 64 + q * 16, u);
-          if constexpr (kBwd) tmem_ld16(acc + 128 + q * 16, dh);
-          tmem_wait_ld(g);
-          tmem_wait_ld(u);
+          float(&g)[16] = v[q & 1][0];
+          float(&u)[16] = v[q & 1][1];
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) tmem_wait_ld(v[q & 1][k]);
+          if (q + 1 < grans) {
+            if (q < 3) {
+#pragma unroll
+              for (int k = 0; k < kParts; ++k)
+                tmem_ld16(acc + 64 * k + 16 * (q + 1), v[(q + 1) & 1][k]);
+            }
+          } else {
+            tc_fence_before();
+            warp_arrive(&bars.gempty[group], lane);  // the accumulators have been read
+          }
+          float s[16];
+          sigmoid16(g, s);
           if constexpr (kBwd) {
-            tmem_wait_ld(dh);
+            float(&dh)[16] = v[q & 1][kParts - 1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float s = sigmoid(g[i]), act = g[i] * s, d = dh[i];
-              dh[i] = d * act;                               // dU
-              g[i] = d * u[i] * (s + act * (1.f - s));       // dG
+              const float act = g[i] * s[i], d = dh[i];
+              dh[i] = d * act;                                   // dU
+              g[i] = d * u[i] * (s[i] + act * (1.f - s[i]));     // dG
             }
             store_granule(hbuf, row, q, g);
             store_granule(hbuf + kBlockBytes, row, q, dh);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) g[i] = g[i] * sigmoid(g[i]) * u[i];
+            for (int i = 0; i < 16; ++i) g[i] = g[i] * s[i] * u[i];
             store_granule(hbuf, row, q, g);
           }
         }
       }
-      tc_fence_before();
       fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&bars.gempty[group]);
-        mbar_arrive(&bars.hfull[group]);
+      warp_arrive(&bars.hfull[group], lane);
+      // while this tile's products run
+      if (share == 2) {
+        if (told < t) output(told++);
+      } else if (j == 0 && it > 0) {
+        output(t - 1);
       }
-      if (j == 0 && it > 0) output(t - 1);  // while this tile's products run
     }
-    if (group == (steps & 1)) output(mine - 1);
-  } else if (warp == 8) {
-    int slot = 0, round = 0;
-    auto acquire = [&](uint32_t fixed) {
+    if (share == 2) {
+      while (told < mine) output(told++);
+    } else if (group == (steps & 1)) {
+      output(mine - 1);
+    }
+  } else if (warp == 8 || warp == 9) {
+    // Position of a step's blocks in the stream of weight blocks: F0, F1 S0,
+    // F2 S1, ... with F and S blocks for a step's first and second products.
+    const int fb = kBwd ? p.cd + wblocks : p.cd, sb = kBwd ? p.cd : wblocks;
+    auto at = [&](int pos) { return p.resident ? 0 : pos % p.slots; };
+    auto acquire = [&](uint32_t fixed, int pos) {
       if (p.resident) return ws + fixed;
-      wait(&bars.wfull[slot], round);
-      return ws + slot * kBlockBytes;
+      wait(&bars.wfull[pos % p.slots], pos / p.slots);
+      return ws + (pos % p.slots) * kBlockBytes;
     };
-    auto release = [&] {
-      if (p.resident) return;
-      tc_commit(&bars.wempty[slot]);
-      if (++slot == p.slots) slot = 0, ++round;
+    auto release = [&](int pos) {
+      if (!p.resident) tc_commit(&bars.wempty[at(pos)]);
     };
-    int j1 = 0, xb = 0, xround = 0;
-    auto first = [&](int it) {
-      const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
-      const uint32_t acc = tmem + (p.nb == 2 ? it & 1 : 0) * kGCols;
-      if (j1 == 0) wait(&bars.xfull[xb], xround);
-      const int before = it - p.nb;
-      if (before >= 0) wait(&bars.gempty[before & 1], before >> 1);
-      tc_fence_after();
-      for (int c = 0; c < p.cd; ++c) {
-        const uint32_t w = acquire(wgu_offset(p, j1, c));
-        tc_mma_steps<4>(acc, desc_k(x + c * kBlockBytes), kStepK, desc_k(w), kStepK,
-                        tc_idesc(128, false, false), p.kd - 4 * c, c > 0);
-        release();
-      }
-      if constexpr (kBwd) {
-        for (int b8 = 0; b8 < wblocks; ++b8) {
-          const uint32_t w = acquire(wd_offset(p, j1, b8));
-          for (int c = 0; c < 2 && 2 * b8 + c < p.co; ++c)
-            tc_mma_steps<4>(acc + 128, desc_k(dy + (2 * b8 + c) * kBlockBytes), kStepK,
-                            desc_mn(w + c * 64 * 128, kBlockBytes), kStepMn,
-                            tc_idesc(64, false, true), p.ko - 8 * b8 - 4 * c, b8 + c > 0);
-          release();
+    if (warp == 8) {
+      int j = 0, xb = 0, xround = 0;
+      for (int it = 0; it < steps; ++it) {
+        int pos = it == 0 ? 0 : fb + (it - 1) * (fb + sb);
+        const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
+        const uint32_t acc = tmem + (p.nb == 2 ? it & 1 : 0) * kGCols;
+        if (j == 0) wait(&bars.xfull[xb], xround);
+        const int before = it - p.nb;
+        if (before >= 0) wait(&bars.gempty[before & 1], before >> 1);
+        tc_fence_after();
+        for (int c = 0; c < p.cd; ++c) {
+          const uint32_t w = acquire(wgu_offset(p, j, c), pos);
+          tc_mma_steps<4>(acc, desc_k(x + c * kBlockBytes), kStepK, desc_k(w), kStepK,
+                          tc_idesc(128, false, false), p.kd - 4 * c, c > 0);
+          release(pos++);
+        }
+        if constexpr (kBwd) {
+          for (int b8 = 0; b8 < wblocks; ++b8) {
+            const uint32_t w = acquire(wd_offset(p, j, b8), pos);
+            for (int c = 0; c < 2 && 2 * b8 + c < p.co; ++c)
+              tc_mma_steps<4>(acc + 128, desc_k(dy + (2 * b8 + c) * kBlockBytes), kStepK,
+                              desc_mn(w + c * 64 * 128, kBlockBytes), kStepMn,
+                              tc_idesc(64, false, true), p.ko - 8 * b8 - 4 * c, b8 + c > 0);
+            release(pos++);
+          }
+        }
+        tc_commit(&bars.gfull[it & 1]);
+        if (++j == p.nc) {
+          tc_commit(&bars.xempty[xb]);
+          j = 0;
+          if (++xb == p.nx) xb = 0, ++xround;
         }
       }
-      tc_commit(&bars.gfull[it & 1]);
-      if (++j1 == p.nc) {
-        tc_commit(&bars.xempty[xb]);
-        j1 = 0;
-        if (++xb == p.nx) xb = 0, ++xround;
-      }
-    };
-    int j = 0, t = 0;
-    first(0);
-    for (int it = 0; it < steps; ++it) {
-      if (it + 1 < steps) first(it + 1);
-      wait(&bars.hfull[it & 1], it >> 1);
-      if (j == 0 && t > 0) wait(&bars.yempty, t - 1);
-      tc_fence_after();
-      const uint32_t h = hs + (p.nh == 2 ? it & 1 : 0) * p.h_bytes;
-      const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
-      if constexpr (kBwd) {
-        // dG Wg + dU Wu: the blocks' columns are N, their rows K
-        const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
-        for (int c = 0; c < p.cd; c += wide) {
-          const uint32_t w = acquire(wgu_offset(p, j, c));
-          const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
-          tc_mma_steps<4>(yacc + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
-                          ks, j > 0);
-          tc_mma_steps<4>(yacc + 64 * c, desc_k(h + kBlockBytes), kStepK,
-                          desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
-          release();
+    } else {
+      int j = 0, t = 0;
+      for (int it = 0; it < steps; ++it) {
+        int pos = it + 1 < steps ? 2 * fb + it * (fb + sb) : fb + it * (fb + sb);
+        wait(&bars.hfull[it & 1], it >> 1);
+        if (j == 0 && t > 0) wait(&bars.yempty, t - 1);
+        tc_fence_after();
+        const uint32_t h = hs + (p.nh == 2 ? it & 1 : 0) * p.h_bytes;
+        const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
+        if constexpr (kBwd) {
+          // dG Wg + dU Wu: the blocks' columns are N, their rows K
+          const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
+          for (int c = 0; c < p.cd; c += wide) {
+            const uint32_t w = acquire(wgu_offset(p, j, c), pos);
+            const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
+            tc_mma_steps<4>(yacc + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
+                            ks, j > 0);
+            tc_mma_steps<4>(yacc + 64 * c, desc_k(h + kBlockBytes), kStepK,
+                            desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
+            release(pos++);
+          }
+        } else {
+          const int wide = p.resident ? wblocks : 1;
+          for (int b8 = 0; b8 < wblocks; b8 += wide) {
+            const uint32_t w = acquire(wd_offset(p, j, b8), pos);
+            tc_mma_steps<4>(yacc + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
+                            tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
+                            j > 0);
+            release(pos++);
+          }
         }
-      } else {
-        const int wide = p.resident ? wblocks : 1;
-        for (int b8 = 0; b8 < wblocks; b8 += wide) {
-          const uint32_t w = acquire(wd_offset(p, j, b8));
-          tc_mma_steps<4>(yacc + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
-                          tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks, j > 0);
-          release();
+        tc_commit(&bars.hempty[it & 1]);
+        if (++j == p.nc) {
+          tc_commit(&bars.yfull[t & 1]);
+          j = 0, ++t;
         }
-      }
-      tc_commit(&bars.hempty[it & 1]);
-      if (++j == p.nc) {
-        tc_commit(&bars.yfull[t & 1]);
-        j = 0, ++t;
       }
     }
     tc_commit(&bars.done);
-    if (!mbar_wait_bounded(&bars.done, 0))
+    if (!tc_wait(&bars.done, 0))
       report_error(p.f.err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
-  } else if (warp == 9) {
+  } else if (warp == 10) {
     if (lane == 0 && !p.resident) {
       int slot = 0, round = 0;
       auto put = [&](uint32_t offset, uint32_t bytes) {
@@ -444,27 +499,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       if (!wait.ok) {  // copies in flight land before the block leaves
         for (int i = 0; i < p.slots; ++i) {
           const int r = i < slot ? round : round - 1;
-          if (r >= 0) mbar_wait_bounded(&bars.wfull[i], r & 1);
+          if (r >= 0) tc_wait(&bars.wfull[i], r & 1);
         }
       }
     }
   } else {
-    const int tid = threadIdx.x - kEpi - 64;
-    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p.f.x);
-    const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(p.f.dy);
+    const bool threads = !p.tma_x || (kBwd && !p.tma_dy);
     int xb = 0, round = 0;
     for (int t = 0; t < mine; ++t) {
       if (round > 0) wait(&bars.xempty[xb], round - 1);
       const int64_t r0 = (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile;
       const uint32_t dst = xs + xb * p.tile_bytes;
-      const bool both = kBwd && !p.tma_dy;
-      if (!p.tma_x) load_tile(dst, x, p.f.x_stride, r0, p.f.n, p.f.d, p.kd, tid);
-      if (both)
-        load_tile(dst + p.cd * kBlockBytes, dy, p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, tid);
-      if (!p.tma_x || both) fence_proxy_async_smem();
-      if (warp == 11) {
+      if (warp > 11) {
+        const int tid = threadIdx.x - kEpi - 128;
+        if (!p.tma_x)
+          load_tile(dst, static_cast<const __nv_bfloat16*>(p.f.x), p.f.x_stride, r0, p.f.n, p.f.d,
+                    p.kd, tid);
+        if (kBwd && !p.tma_dy)
+          load_tile(dst + p.cd * kBlockBytes, static_cast<const __nv_bfloat16*>(p.f.dy),
+                    p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, tid);
+        if (threads) fence_proxy_async_smem();
         warp_arrive(&bars.xfull[xb], lane);
-      } else if (__syncwarp(), lane == 0 && wait.ok) {
+      } else if (lane == 0 && wait.ok) {
         const int xblocks = p.tma_x ? p.cd : 0, yblocks = kBwd && p.tma_dy ? p.co : 0;
         mbar_arrive_expect_tx(&bars.xfull[xb], (xblocks + yblocks) * kBlockBytes);
         for (int c = 0; c < xblocks; ++c)
@@ -476,10 +532,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       }
       if (++xb == p.nx) xb = 0, ++round;
     }
-    if (tid == 0 && !wait.ok) {  // copies in flight land before the block leaves
+    if (warp == 11 && lane == 0 && !wait.ok) {  // copies in flight land before the block leaves
       for (int i = 0; i < p.nx; ++i) {
         const int r = i < xb ? round : round - 1;
-        if (r >= 0) mbar_wait_bounded(&bars.xfull[i], r & 1);
+        if (r >= 0) tc_wait(&bars.xfull[i], r & 1);
       }
     }
   }

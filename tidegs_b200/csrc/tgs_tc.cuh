@@ -46,6 +46,20 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool a_mn, bool b_mn) {
          (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// Waits for `phase` of `bar`, at most 2^22 probes and about two seconds (a
+// probe may itself sleep for a while, so their number alone bounds little).
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t phase) {
+  if (mbar_try_wait(bar, phase)) return true;
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
+  for (uint32_t it = 0; it < kWaitLimit; ++it) {
+    if (mbar_try_wait(bar, phase)) return true;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+    if (now - start > 2000000000ull) return false;
+  }
+  return false;
+}
+
 // One lane of the (converged) warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t on;
@@ -81,9 +95,15 @@ __device__ __forceinline__ void tc_mma_steps(uint32_t acc, uint32_t a, uint32_t 
                                              uint32_t b_step, uint32_t idesc, int steps,
                                              bool accumulate) {
   if (elect_one()) {
+    if (steps >= kMost) {  // most often: no branch between the instructions
 #pragma unroll
-    for (int k = 0; k < kMost; ++k)
-      if (k < steps) tc_mma(acc, a + k * a_step, b + k * b_step, idesc, accumulate || k > 0);
+      for (int k = 0; k < kMost; ++k)
+        tc_mma(acc, a + k * a_step, b + k * b_step, idesc, accumulate || k > 0);
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < steps; ++k)
+        tc_mma(acc, a + k * a_step, b + k * b_step, idesc, accumulate || k > 0);
+    }
   }
   __syncwarp();
 }
