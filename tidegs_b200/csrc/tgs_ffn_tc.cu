@@ -8,12 +8,12 @@
 // products add that chunk's share to the output tile's accumulators (Y, or
 // dX). The roles are warps of their own joined by mbarriers, so loads,
 // products and the activation of different chunks run at once:
-//   warps 0-7    activation, output: two groups of four take turns by chunk
-//   warps 8, 9   issue the first and the second products (a warp each: the
+//   warps 0-15   activation: two groups of eight take turns by chunk
+//   warps 16, 17 issue the first and the second products (a warp each: the
 //                next chunk's first products do not wait behind the output)
-//   warp  10     weight blocks (bulk copies)
-//   warp  11     row tiles by tensor-map copies
-//   warps 12-15  row tiles that no tensor map describes
+//   warp  18     weight blocks (bulk copies)
+//   warp  19     row tiles by tensor-map copies
+//   warps 20-23  the output tile; row tiles that no tensor map describes
 // The same block of weights serves both products: as K-major operand of one
 // and as MN-major operand of the other.
 //
@@ -28,12 +28,14 @@
 namespace tgs {
 namespace {
 
-constexpr int kEpi = 256;      // activation threads
-constexpr int kLoad = 128;     // threads for rows that no tensor map describes
+constexpr int kEpi = 512;      // activation threads, in two groups
+constexpr int kLoad = 128;     // threads of the output, and of rows that no tensor map describes
 constexpr int kTcThreads = kEpi + 128 + kLoad;
+constexpr int kWarpF = kEpi / 32, kWarpS = kWarpF + 1, kWarpW = kWarpF + 2, kWarpT = kWarpF + 3;
 constexpr int kTile = 128;     // rows
 constexpr int kChunk = 64;     // hidden values
 constexpr int kMaxTiles = 3;   // row-tile buffers
+constexpr int kMaxHid = 4;     // hidden buffers
 constexpr int kMaxSlots = 12;  // weight ring
 constexpr int kSmemBudget = 227 * 1024 - 2048;  // less alignment and barriers
 
@@ -44,7 +46,8 @@ struct TcParams {
   int64_t tiles;
   int cd, co, nc;  // operand blocks of D and O, chunks of H
   int kd, ko;      // 16-steps of D and O
-  int nx, nh, nb, slots;
+  int nx, nh, nb, ny, slots;  // buffers: row tiles, hidden, first and output accumulators
+  int ycols;                  // columns of one output accumulator
   int resident, tma_x, tma_dy, vec_y;
   uint32_t tile_bytes, h_bytes, w_bytes;
   uint32_t tmem_cols;
@@ -52,8 +55,8 @@ struct TcParams {
 
 struct TcBars {
   uint64_t xfull[kMaxTiles], xempty[kMaxTiles];
-  uint64_t gfull[2], gempty[2], hfull[2], hempty[2];
-  uint64_t yfull[2], yempty, done;
+  uint64_t gfull[2], gempty[2], hfull[kMaxHid], hempty[kMaxHid];
+  uint64_t yfull[2], yempty[2], done;
   uint64_t wfull[kMaxSlots], wempty[kMaxSlots];
   uint32_t tmem;
 };
@@ -149,43 +152,82 @@ __device__ __forceinline__ float fast_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ float sigmoid(float g) {
-  return fast_rcp(1.f + fast_exp2(g * -1.4426950408889634f));
+// Two fp32 values in a register pair: one instruction for both.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2(float a, float b) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  }
+  __device__ __forceinline__ explicit F2(uint64_t x) : v(x) {}
+  __device__ __forceinline__ void get(float& a, float& b) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+  return F2(r);
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+  return F2(r);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return F2(r);
 }
 
-// s[i] = 1 / (1 + exp(-g[i])). The special-function unit (16 results a cycle
-// and SM) bounds the activation, so two values share a reciprocal, 1 / a =
-// b / (a b): 1.5 of its operations a value instead of 2. Where a product
-// leaves the range (g below -43, infinity, NaN) the values get one each.
-__device__ __forceinline__ void sigmoid16(const float (&g)[16], float (&s)[16]) {
-  bool wide = false;
+// 1 / (1 + exp(-g)) of two values. The special-function unit (16 results a
+// cycle and SM) bounds the activation, so they share a reciprocal, 1 / a =
+// b / (a b): 1.5 of its operations a value instead of 2. Where the product
+// leaves the range (g below -43, infinity, NaN) `far` is set and the caller
+// comes back with kEach, for one reciprocal each.
+template <bool kEach>
+__device__ __forceinline__ F2 sigmoid2(F2 g, bool& far) {
+  float ea, eb, a, b;
+  (g * F2(-1.4426950408889634f, -1.4426950408889634f)).get(ea, eb);
+  (F2(fast_exp2(ea), fast_exp2(eb)) + F2(1.f, 1.f)).get(a, b);
+  if constexpr (kEach) return F2(fast_rcp(a), fast_rcp(b));
+  const float ab = a * b, r = fast_rcp(ab);
+  far |= !(ab < 0x1p126f);
+  return F2(r * b, r * a);
+}
+
+// 16 hidden values of a row, rounded and packed in pairs: act(G) U, or dG in
+// `p` and dU in `q`.
+template <bool kBwd, bool kEach>
+__device__ __forceinline__ bool activate(const float (&g)[16], const float (&u)[16],
+                                         const float (&dh)[16], uint32_t (&p)[8],
+                                         uint32_t (&q)[8]) {
+  bool far = false;
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
-    const float a = 1.f + fast_exp2(g[i] * -1.4426950408889634f);
-    const float b = 1.f + fast_exp2(g[i + 1] * -1.4426950408889634f);
-    const float ab = a * b;
-    wide |= !(ab < 0x1p126f);
-    const float r = fast_rcp(ab);
-    s[i] = r * b, s[i + 1] = r * a;
+    const F2 g2(g[i], g[i + 1]), u2(u[i], u[i + 1]), s2 = sigmoid2<kEach>(g2, far);
+    const F2 act = g2 * s2;
+    float a, b;
+    if constexpr (kBwd) {
+      const F2 d2(dh[i], dh[i + 1]);
+      // silu'(g) = s + act (1 - s)
+      const F2 slope = fma2(act, fma2(s2, F2(-1.f, -1.f), F2(1.f, 1.f)), s2);
+      (d2 * u2 * slope).get(a, b);
+      p[i / 2] = pack_bf16(a, b);
+      (d2 * act).get(a, b);
+      q[i / 2] = pack_bf16(a, b);
+    } else {
+      (act * u2).get(a, b);
+      p[i / 2] = pack_bf16(a, b);
+    }
   }
-  if (wide) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = sigmoid(g[i]);
-  }
+  return far;
 }
 
-// Writes 16 values as bf16 into units 2 g16 and 2 g16 + 1 of a block's row.
+// Puts them into units 2 g16 and 2 g16 + 1 of a block's row.
 __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint32_t g16,
-                                              const float (&v)[16]) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint4 q;
-    q.x = pack_bf16(v[8 * half + 0], v[8 * half + 1]);
-    q.y = pack_bf16(v[8 * half + 2], v[8 * half + 3]);
-    q.z = pack_bf16(v[8 * half + 4], v[8 * half + 5]);
-    q.w = pack_bf16(v[8 * half + 6], v[8 * half + 7]);
-    st_shared16(block + unit_offset(row, 2 * g16 + half), q);
-  }
+                                              const uint32_t (&v)[8]) {
+  st_shared16(block + unit_offset(row, 2 * g16), make_uint4(v[0], v[1], v[2], v[3]));
+  st_shared16(block + unit_offset(row, 2 * g16 + 1), make_uint4(v[4], v[5], v[6], v[7]));
 }
 
 // A row tile -> operand blocks, by threads: for matrices that no tensor map
@@ -209,10 +251,10 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src
 }
 
 __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, int64_t tile,
-                                             int out, int lane_row, int from, int step) {
+                                             int out, int lane_row) {
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.f.y);
   const int64_t row = tile * kTile + lane_row;
-  for (int c = from; c < out; c += step) {
+  for (int c = 0; c < out; c += 16) {
     float v[16];
     tmem_ld16(acc + c, v);
     tmem_wait_ld(v);
@@ -256,16 +298,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   constexpr uint32_t kGCols = kBwd ? 192 : 128;
   Waits wait{p.f.err};
 
-  if (warp == 8) {
+  if (warp == kWarpF) {
     tmem_alloc(&bars.tmem, p.tmem_cols);
     if (lane == 0) {
-      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], 1 + kLoad / 32), mbar_init(&bars.xempty[i], 1);
+      const int arrivals = 1 + (!p.tma_x || (kBwd && !p.tma_dy) ? kLoad / 32 : 0);
+      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], arrivals), mbar_init(&bars.xempty[i], 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], 4);
-        mbar_init(&bars.hfull[i], 4), mbar_init(&bars.hempty[i], 1);
-        mbar_init(&bars.yfull[i], 1);
+        mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], kEpi / 64);
+        mbar_init(&bars.yfull[i], 1), mbar_init(&bars.yempty[i], kLoad / 32);
       }
-      mbar_init(&bars.yempty, p.nc > 1 && p.nh == 2 ? 8 : 4), mbar_init(&bars.done, 2);
+      for (int i = 0; i < kMaxHid; ++i) mbar_init(&bars.hfull[i], kEpi / 64), mbar_init(&bars.hempty[i], 1);
+      mbar_init(&bars.done, 2);
       for (int i = 0; i < kMaxSlots; ++i) mbar_init(&bars.wfull[i], 1), mbar_init(&bars.wempty[i], 1);
       fence_mbar_init();
     }
@@ -284,97 +327,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   const uint32_t tmem = bars.tmem;
   const uint32_t yacc = tmem + p.nb * kGCols;
 
-  // Step `it` (tile it / nc, chunk it % nc) signals on the barriers of its
-  // parity, whether or not there are two buffers: each side then meets every
-  // phase of a barrier in turn.
-  if (warp < 8) {
-    // Activation: group warp / 4 takes the steps of its parity; this thread's
-    // row of the tile.
+  // Step `it` (tile it / nc, chunk it % nc) signals on the barriers it % 2, and
+  // it % hm for the hidden buffers, a tile t on those of t % 2, whether or not
+  // there are two buffers: a wait then never meets a barrier that is two phases
+  // from the awaited one, which it could not tell from it.
+  const int hm = max(p.nh, 2);
+  if (warp < kWarpF) {
+    // Activation: group warp / 8 takes the steps of its parity; this thread's
+    // row of the tile, and the 16-column granules half, half + 2 of the chunk.
     const uint32_t row = (warp & 3) * 32 + lane;
-    const int group = warp >> 2;
+    const int group = warp >> 3, half = warp >> 2 & 1;
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane 32 (warp % 4)
     int j = group;
-    const int out = kBwd ? p.f.d : p.f.o;
-    // A tile's output is stored by both groups, every second granule each,
-    // after their first step in the next tile; of one chunk to a tile, or with
-    // one hidden buffer (where a group's step waits for products that wait for
-    // that output), by the group that has the next tile's first step.
-    const int share = p.nc > 1 && p.nh == 2 ? 2 : 1;
-    auto output = [&](int t) {
-      wait(&bars.yfull[t & 1], t >> 1);
-      tc_fence_after();
-      store_output(p, yacc + quarter, blockIdx.x + static_cast<int64_t>(t) * gridDim.x, out, row,
-                   share == 2 ? group * 16 : 0, share * 16);
-      tc_fence_before();
-      warp_arrive(&bars.yempty, lane);
-    };
-    int told = 0;  // tiles whose output this group has stored (share 2)
-    for (int it = group, t = 0; it < steps; it += 2, j += 2) {
-      while (j >= p.nc) j -= p.nc, ++t;
+    int hb = group, hphase = 0;
+    for (int it = group; it < steps; it += 2, j += 2, hb += 2) {
+      while (j >= p.nc) j -= p.nc;
+      if (hb >= hm) hb -= hm, ++hphase;
       wait(&bars.gfull[group], it >> 1);
       tc_fence_after();
       const uint32_t acc = tmem + (p.nb == 2 ? group : 0) * kGCols + quarter;
-      const uint32_t hbuf = hs + (p.nh == 2 ? group : 0) * p.h_bytes;
+      const uint32_t hbuf = hs + (p.nh > 1 ? hb : 0) * p.h_bytes;
       const int grans = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
-      const int before = it - p.nh;  // the step that last used the hidden buffer
-      if (before >= 0) wait(&bars.hempty[before & 1], before >> 1);
-      // Granules of 16 columns; the next one is on its way from tensor memory
-      // while one is computed.
       constexpr int kParts = kBwd ? 3 : 2;  // G, U, dH
-      float v[2][kParts][16];
 #pragma unroll
-      for (int k = 0; k < kParts; ++k) tmem_ld16(acc + 64 * k, v[0][k]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int i = 0; i < 2; ++i) {
+        const int q = half + 2 * i;
+        float v[kParts][16];
         if (q < grans) {
-          float(&g)[16] = v[q & 1][0];
-          float(&u)[16] = v[q & 1][1];
 #pragma unroll
-          for (int k = 0; k < kParts; ++k) tmem_wait_ld(v[q & 1][k]);
-          if (q + 1 < grans) {
-            if (q < 3) {
-#pragma unroll
-              for (int k = 0; k < kParts; ++k)
-                tmem_ld16(acc + 64 * k + 16 * (q + 1), v[(q + 1) & 1][k]);
-            }
-          } else {
-            tc_fence_before();
-            warp_arrive(&bars.gempty[group], lane);  // the accumulators have been read
+          for (int k = 0; k < kParts; ++k) tmem_ld16(acc + 64 * k + 16 * q, v[k]);
+        }
+        if (i == 0) {  // meanwhile: the step that last used the hidden buffer
+          if (p.nh > 1) {
+            if (hphase > 0) wait(&bars.hempty[hb], hphase - 1);
+          } else if (it > 0) {
+            wait(&bars.hempty[(it - 1) & 1], (it - 1) >> 1);
           }
-          float s[16];
-          sigmoid16(g, s);
-          if constexpr (kBwd) {
-            float(&dh)[16] = v[q & 1][kParts - 1];
+        }
+        if (q < grans) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float act = g[i] * s[i], d = dh[i];
-              dh[i] = d * act;                                   // dU
-              g[i] = d * u[i] * (s[i] + act * (1.f - s[i]));     // dG
-            }
-            store_granule(hbuf, row, q, g);
-            store_granule(hbuf + kBlockBytes, row, q, dh);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) g[i] = g[i] * s[i] * u[i];
-            store_granule(hbuf, row, q, g);
-          }
+          for (int k = 0; k < kParts; ++k) tmem_wait_ld(v[k]);
+        }
+        if (i == 1) {
+          tc_fence_before();
+          warp_arrive(&bars.gempty[group], lane);  // the accumulators have been read
+        }
+        if (q < grans) {
+          uint32_t h0[8], h1[8];
+          if (activate<kBwd, kBwd>(v[0], v[1], v[kParts - 1], h0, h1))
+            activate<kBwd, true>(v[0], v[1], v[kParts - 1], h0, h1);
+          store_granule(hbuf, row, q, h0);
+          if constexpr (kBwd) store_granule(hbuf + kBlockBytes, row, q, h1);
         }
       }
       fence_proxy_async_smem();
-      warp_arrive(&bars.hfull[group], lane);
-      // while this tile's products run
-      if (share == 2) {
-        if (told < t) output(told++);
-      } else if (j == 0 && it > 0) {
-        output(t - 1);
-      }
+      warp_arrive(&bars.hfull[hb], lane);
     }
-    if (share == 2) {
-      while (told < mine) output(told++);
-    } else if (group == (steps & 1)) {
-      output(mine - 1);
-    }
-  } else if (warp == 8 || warp == 9) {
+  } else if (warp == kWarpF || warp == kWarpS) {
     // Position of a step's blocks in the stream of weight blocks: F0, F1 S0,
     // F2 S1, ... with F and S blocks for a step's first and second products.
     const int fb = kBwd ? p.cd + wblocks : p.cd, sb = kBwd ? p.cd : wblocks;
@@ -387,7 +396,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
     auto release = [&](int pos) {
       if (!p.resident) tc_commit(&bars.wempty[at(pos)]);
     };
-    if (warp == 8) {
+    if (warp == kWarpF) {
       int j = 0, xb = 0, xround = 0;
       for (int it = 0; it < steps; ++it) {
         int pos = it == 0 ? 0 : fb + (it - 1) * (fb + sb);
@@ -421,13 +430,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         }
       }
     } else {
-      int j = 0, t = 0;
+      int j = 0, t = 0, hb = 0, hphase = 0;
       for (int it = 0; it < steps; ++it) {
         int pos = it + 1 < steps ? 2 * fb + it * (fb + sb) : fb + it * (fb + sb);
-        wait(&bars.hfull[it & 1], it >> 1);
-        if (j == 0 && t > 0) wait(&bars.yempty, t - 1);
+        wait(&bars.hfull[hb], hphase);
+        if (j == 0 && t >= p.ny) wait(&bars.yempty[(t - p.ny) & 1], (t - p.ny) >> 1);
         tc_fence_after();
-        const uint32_t h = hs + (p.nh == 2 ? it & 1 : 0) * p.h_bytes;
+        const uint32_t y = yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols;
+        const uint32_t h = hs + (p.nh > 1 ? hb : 0) * p.h_bytes;
         const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
         if constexpr (kBwd) {
           // dG Wg + dU Wu: the blocks' columns are N, their rows K
@@ -435,9 +445,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
           for (int c = 0; c < p.cd; c += wide) {
             const uint32_t w = acquire(wgu_offset(p, j, c), pos);
             const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
-            tc_mma_steps<4>(yacc + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
+            tc_mma_steps<4>(y + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
                             ks, j > 0);
-            tc_mma_steps<4>(yacc + 64 * c, desc_k(h + kBlockBytes), kStepK,
+            tc_mma_steps<4>(y + 64 * c, desc_k(h + kBlockBytes), kStepK,
                             desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
             release(pos++);
           }
@@ -445,13 +455,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
           const int wide = p.resident ? wblocks : 1;
           for (int b8 = 0; b8 < wblocks; b8 += wide) {
             const uint32_t w = acquire(wd_offset(p, j, b8), pos);
-            tc_mma_steps<4>(yacc + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
+            tc_mma_steps<4>(y + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
                             tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
                             j > 0);
             release(pos++);
           }
         }
-        tc_commit(&bars.hempty[it & 1]);
+        tc_commit(&bars.hempty[hb]);
+        if (++hb == hm) hb = 0, ++hphase;
         if (++j == p.nc) {
           tc_commit(&bars.yfull[t & 1]);
           j = 0, ++t;
@@ -461,7 +472,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
     tc_commit(&bars.done);
     if (!tc_wait(&bars.done, 0))
       report_error(p.f.err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
-  } else if (warp == 10) {
+  } else if (warp == kWarpW) {
     if (lane == 0 && !p.resident) {
       int slot = 0, round = 0;
       auto put = [&](uint32_t offset, uint32_t bytes) {
@@ -503,24 +514,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         }
       }
     }
-  } else {
-    const bool threads = !p.tma_x || (kBwd && !p.tma_dy);
-    int xb = 0, round = 0;
-    for (int t = 0; t < mine; ++t) {
-      if (round > 0) wait(&bars.xempty[xb], round - 1);
-      const int64_t r0 = (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile;
-      const uint32_t dst = xs + xb * p.tile_bytes;
-      if (warp > 11) {
-        const int tid = threadIdx.x - kEpi - 128;
-        if (!p.tma_x)
-          load_tile(dst, static_cast<const __nv_bfloat16*>(p.f.x), p.f.x_stride, r0, p.f.n, p.f.d,
-                    p.kd, tid);
-        if (kBwd && !p.tma_dy)
-          load_tile(dst + p.cd * kBlockBytes, static_cast<const __nv_bfloat16*>(p.f.dy),
-                    p.f.dy_stride, r0, p.f.n, p.f.o, p.ko, tid);
-        if (threads) fence_proxy_async_smem();
-        warp_arrive(&bars.xfull[xb], lane);
-      } else if (lane == 0 && wait.ok) {
+  } else if (warp == kWarpT) {
+    if (lane == 0) {
+      int xb = 0, round = 0;
+      for (int t = 0; t < mine && wait.ok; ++t) {
+        if (round > 0) wait(&bars.xempty[xb], round - 1);
+        if (!wait.ok) break;
+        const int64_t r0 = (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile;
+        const uint32_t dst = xs + xb * p.tile_bytes;
         const int xblocks = p.tma_x ? p.cd : 0, yblocks = kBwd && p.tma_dy ? p.co : 0;
         mbar_arrive_expect_tx(&bars.xfull[xb], (xblocks + yblocks) * kBlockBytes);
         for (int c = 0; c < xblocks; ++c)
@@ -529,20 +530,54 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         for (int c = 0; c < yblocks; ++c)
           tma_load_2d(dst + (p.cd + c) * kBlockBytes, &p.dymap, c * kBlockCols,
                       static_cast<int>(r0), &bars.xfull[xb]);
+        if (++xb == p.nx) xb = 0, ++round;
       }
-      if (++xb == p.nx) xb = 0, ++round;
+      if (!wait.ok) {  // copies in flight land before the block leaves
+        for (int i = 0; i < p.nx; ++i) {
+          const int r = i < xb ? round : round - 1;
+          if (r >= 0) tc_wait(&bars.xfull[i], r & 1);
+        }
+      }
     }
-    if (warp == 11 && lane == 0 && !wait.ok) {  // copies in flight land before the block leaves
-      for (int i = 0; i < p.nx; ++i) {
-        const int r = i < xb ? round : round - 1;
-        if (r >= 0) tc_wait(&bars.xfull[i], r & 1);
+  } else {
+    const bool tx = !p.tma_x, ty = kBwd && !p.tma_dy;
+    const int tid = threadIdx.x - kEpi - 128;
+    const int out = kBwd ? p.f.d : p.f.o;
+    const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;
+    auto row_of = [&](int t) { return (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile; };
+    int xb = 0, round = 0;
+    // Loads run nx tiles ahead of the output: the buffer that a load waits for
+    // is then never one whose tile waits for this output.
+    const int ahead = tx || ty ? p.nx : 0;
+    for (int t = 0; t < mine + ahead; ++t) {
+      if (ahead && t < mine) {
+        if (round > 0) wait(&bars.xempty[xb], round - 1);
+        const uint32_t dst = xs + xb * p.tile_bytes;
+        if (tx)
+          load_tile(dst, static_cast<const __nv_bfloat16*>(p.f.x), p.f.x_stride, row_of(t), p.f.n,
+                    p.f.d, p.kd, tid);
+        if (ty)
+          load_tile(dst + p.cd * kBlockBytes, static_cast<const __nv_bfloat16*>(p.f.dy),
+                    p.f.dy_stride, row_of(t), p.f.n, p.f.o, p.ko, tid);
+        fence_proxy_async_smem();
+        warp_arrive(&bars.xfull[xb], lane);
+        if (++xb == p.nx) xb = 0, ++round;
+      }
+      const int done = t - ahead;
+      if (done >= 0) {
+        wait(&bars.yfull[done & 1], done >> 1);
+        tc_fence_after();
+        store_output(p, yacc + (p.ny == 2 ? done & 1 : 0) * p.ycols + quarter,
+                     row_of(done) / kTile, out, (warp & 3) * 32 + lane);
+        tc_fence_before();
+        warp_arrive(&bars.yempty[done & 1], lane);
       }
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kWarpF) {
     tc_fence_after();
     tmem_free(tmem, p.tmem_cols);
   }
@@ -583,15 +618,19 @@ void plan_rows(TcParams& p, bool bwd) {
   p.h_bytes = (bwd ? 2 : 1) * kBlockBytes;
   const uint32_t out = bwd ? p.kd * 16 : p.ko * 16, g = bwd ? 192 : 128;
   p.nb = 2 * g + out <= 512 ? 2 : 1;
-  p.tmem_cols = pow2_cols(p.nb * g + out);
+  p.ny = p.nb * g + 2 * out <= 512 ? 2 : 1;
+  p.ycols = out;
+  p.tmem_cols = pow2_cols(p.nb * g + p.ny * out);
   const int64_t budget = kSmemBudget;
   auto used = [&] { return static_cast<int64_t>(p.nx) * p.tile_bytes + p.nh * p.h_bytes; };
   p.nx = 2, p.nh = 2, p.slots = 1;
   p.resident = used() + p.w_bytes <= budget;
   if (p.resident) {
-    p.nx = 3;
-    if (used() + p.w_bytes > budget) p.nx = 2;
-    return;
+    for (int nh = kMaxHid; nh >= 2; --nh) {
+      p.nh = nh;
+      for (p.nx = 3; p.nx >= 2; --p.nx)
+        if (used() + p.w_bytes <= budget) return;
+    }
   }
   // The ring holds at least one chunk's blocks twice over before a second
   // row tile or hidden buffer is bought with it.
@@ -611,6 +650,11 @@ uint32_t rows_smem(const TcParams& p) {
 template <bool kBwd>
 int launch_tc_rows(TcParams p, cudaStream_t s) {
   plan_rows(p, kBwd);
+  const int smem = static_cast<int>(rows_smem(p));
+  // Before the tensor maps: this binds the thread's context, which a thread of
+  // autograd's may not have yet and the encoder needs.
+  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_rows_kernel<kBwd>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (int rc = make_maps(p, kBwd)) return rc;
   const int out = kBwd ? p.f.d : p.f.o;
   p.vec_y = out % 8 == 0 && aligned16(p.f.y);
@@ -620,9 +664,6 @@ int launch_tc_rows(TcParams p, cudaStream_t s) {
     ffn_pack_kernel<<<ceil_div<uint32_t>(p.w_bytes / 16, 256), 256, 0, s>>>(p, packed);
     TGS_LAUNCH_CHECK();
   }
-  const int smem = static_cast<int>(rows_smem(p));
-  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_rows_kernel<kBwd>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int grid = static_cast<int>(std::min<int64_t>(p.tiles, sm_count()));
   ffn_tc_rows_kernel<kBwd><<<grid, kTcThreads, smem, s>>>(p);
   TGS_LAUNCH_CHECK();
