@@ -265,7 +265,9 @@ def test_gated_feed_forward(dtype, n, d, h, o):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("n,d,h,o", [(40003, 32, 64, 3), (30011, 64, 128, 48), (20000, 128, 160, 96)])
+@pytest.mark.parametrize("n,d,h,o", [(40003, 32, 64, 3), (30011, 64, 128, 48), (20000, 128, 160, 96),
+                                     (60000, 256, 192, 256), (50000, 130, 129, 200), (60000, 200, 100, 16),
+                                     (60000, 16, 60, 256), (60000, 33, 64, 35)])
 def test_gated_feed_forward_many_rows(dtype, n, d, h, o):
     _ffn_check(*_ffn_inputs(n, d, h, o, dtype))
 

@@ -46,7 +46,7 @@ struct TcParams {
   int64_t tiles;
   int cd, co, nc;  // operand blocks of D and O, chunks of H
   int kd, ko;      // 16-steps of D and O
-  int nx, nh, nb, ny, slots;  // buffers: row tiles, hidden, first and output accumulators
+  int nx, nh, nb, ny, slots, slots_f;  // buffers: row tiles, hidden, first and output accumulators
   int ycols;                  // columns of one output accumulator
   int resident, tma_x, tma_dy, vec_y;
   uint32_t tile_bytes, h_bytes, w_bytes;
@@ -384,22 +384,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       warp_arrive(&bars.hfull[hb], lane);
     }
   } else if (warp == kWarpF || warp == kWarpS) {
-    // Position of a step's blocks in the stream of weight blocks: F0, F1 S0,
-    // F2 S1, ... with F and S blocks for a step's first and second products.
-    const int fb = kBwd ? p.cd + wblocks : p.cd, sb = kBwd ? p.cd : wblocks;
-    auto at = [&](int pos) { return p.resident ? 0 : pos % p.slots; };
-    auto acquire = [&](uint32_t fixed, int pos) {
+    // Each warp has a ring of its own (of one ring, each would miss phases).
+    const int ring = warp == kWarpF ? 0 : p.slots_f;
+    const int ring_end = warp == kWarpF ? p.slots_f : p.slots;
+    int slot = ring, wround = 0;
+    auto acquire = [&](uint32_t fixed) {
       if (p.resident) return ws + fixed;
-      wait(&bars.wfull[pos % p.slots], pos / p.slots);
-      return ws + (pos % p.slots) * kBlockBytes;
+      wait(&bars.wfull[slot], wround);
+      return ws + slot * kBlockBytes;
     };
-    auto release = [&](int pos) {
-      if (!p.resident) tc_commit(&bars.wempty[at(pos)]);
+    auto release = [&] {
+      if (p.resident) return;
+      tc_commit(&bars.wempty[slot]);
+      if (++slot == ring_end) slot = ring, ++wround;
     };
     if (warp == kWarpF) {
       int j = 0, xb = 0, xround = 0;
       for (int it = 0; it < steps; ++it) {
-        int pos = it == 0 ? 0 : fb + (it - 1) * (fb + sb);
         const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
         const uint32_t acc = tmem + (p.nb == 2 ? it & 1 : 0) * kGCols;
         if (j == 0) wait(&bars.xfull[xb], xround);
@@ -407,19 +408,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         if (before >= 0) wait(&bars.gempty[before & 1], before >> 1);
         tc_fence_after();
         for (int c = 0; c < p.cd; ++c) {
-          const uint32_t w = acquire(wgu_offset(p, j, c), pos);
+          const uint32_t w = acquire(wgu_offset(p, j, c));
           tc_mma_steps<4>(acc, desc_k(x + c * kBlockBytes), kStepK, desc_k(w), kStepK,
                           tc_idesc(128, false, false), p.kd - 4 * c, c > 0);
-          release(pos++);
+          release();
         }
         if constexpr (kBwd) {
           for (int b8 = 0; b8 < wblocks; ++b8) {
-            const uint32_t w = acquire(wd_offset(p, j, b8), pos);
+            const uint32_t w = acquire(wd_offset(p, j, b8));
             for (int c = 0; c < 2 && 2 * b8 + c < p.co; ++c)
               tc_mma_steps<4>(acc + 128, desc_k(dy + (2 * b8 + c) * kBlockBytes), kStepK,
                               desc_mn(w + c * 64 * 128, kBlockBytes), kStepMn,
                               tc_idesc(64, false, true), p.ko - 8 * b8 - 4 * c, b8 + c > 0);
-            release(pos++);
+            release();
           }
         }
         tc_commit(&bars.gfull[it & 1]);
@@ -432,7 +433,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
     } else {
       int j = 0, t = 0, hb = 0, hphase = 0;
       for (int it = 0; it < steps; ++it) {
-        int pos = it + 1 < steps ? 2 * fb + it * (fb + sb) : fb + it * (fb + sb);
         wait(&bars.hfull[hb], hphase);
         if (j == 0 && t >= p.ny) wait(&bars.yempty[(t - p.ny) & 1], (t - p.ny) >> 1);
         tc_fence_after();
@@ -443,22 +443,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
           // dG Wg + dU Wu: the blocks' columns are N, their rows K
           const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
           for (int c = 0; c < p.cd; c += wide) {
-            const uint32_t w = acquire(wgu_offset(p, j, c), pos);
+            const uint32_t w = acquire(wgu_offset(p, j, c));
             const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
             tc_mma_steps<4>(y + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
                             ks, j > 0);
             tc_mma_steps<4>(y + 64 * c, desc_k(h + kBlockBytes), kStepK,
                             desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
-            release(pos++);
+            release();
           }
         } else {
           const int wide = p.resident ? wblocks : 1;
           for (int b8 = 0; b8 < wblocks; b8 += wide) {
-            const uint32_t w = acquire(wd_offset(p, j, b8), pos);
+            const uint32_t w = acquire(wd_offset(p, j, b8));
             tc_mma_steps<4>(y + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
                             tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
                             j > 0);
-            release(pos++);
+            release();
           }
         }
         tc_commit(&bars.hempty[hb]);
@@ -474,34 +474,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       report_error(p.f.err, TGS_DEV_WAIT_TIMEOUT, blockIdx.x, threadIdx.x);
   } else if (warp == kWarpW) {
     if (lane == 0 && !p.resident) {
-      int slot = 0, round = 0;
-      auto put = [&](uint32_t offset, uint32_t bytes) {
-        if (round > 0) wait(&bars.wempty[slot], round - 1);
+      struct Ring {
+        int begin, end, slot, round;
+      } first{0, p.slots_f, 0, 0}, second{p.slots_f, p.slots, p.slots_f, 0};
+      auto put = [&](Ring& r, uint32_t offset, uint32_t bytes) {
+        if (r.round > 0) wait(&bars.wempty[r.slot], r.round - 1);
         if (!wait.ok) return;  // after a wait that ran out, no copy may land in a slot in use
-        mbar_arrive_expect_tx(&bars.wfull[slot], bytes);
-        bulk_g2s(raw + (ws - smem_addr(raw)) + slot * kBlockBytes, p.packed + offset, bytes,
-                 &bars.wfull[slot]);
-        if (++slot == p.slots) slot = 0, ++round;
+        mbar_arrive_expect_tx(&bars.wfull[r.slot], bytes);
+        bulk_g2s(raw + (ws - smem_addr(raw)) + r.slot * kBlockBytes, p.packed + offset, bytes,
+                 &bars.wfull[r.slot]);
+        if (++r.slot == r.end) r.slot = r.begin, ++r.round;
       };
-      auto put_gu = [&](int j) {
-        for (int c = 0; c < p.cd; ++c) put(wgu_offset(p, j, c), kBlockBytes);
+      auto put_gu = [&](Ring& r, int j) {
+        for (int c = 0; c < p.cd; ++c) put(r, wgu_offset(p, j, c), kBlockBytes);
       };
-      auto put_d = [&](int j) {
+      auto put_d = [&](Ring& r, int j) {
         for (int b8 = 0; b8 < wblocks; ++b8)
-          put(wd_offset(p, j, b8), min(8, p.ko - 8 * b8) * 2048);
+          put(r, wd_offset(p, j, b8), min(8, p.ko - 8 * b8) * 2048);
       };
+      // F0, F1 S0, F2 S1, ...: no first products wait for blocks that only come
+      // after those of a second product that waits for them.
       int j1 = 0, j = 0;
       for (int it = -1; it < steps; ++it) {
         if (it + 1 < steps) {
-          put_gu(j1);
-          if (kBwd) put_d(j1);
+          put_gu(first, j1);
+          if (kBwd) put_d(first, j1);
           if (++j1 == p.nc) j1 = 0;
         }
         if (it >= 0) {
           if (kBwd) {
-            put_gu(j);
+            put_gu(second, j);
           } else {
-            put_d(j);
+            put_d(second, j);
           }
           if (++j == p.nc) j = 0;
         }
@@ -509,7 +513,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       }
       if (!wait.ok) {  // copies in flight land before the block leaves
         for (int i = 0; i < p.slots; ++i) {
-          const int r = i < slot ? round : round - 1;
+          const Ring& g = i < p.slots_f ? first : second;
+          const int r = i < g.slot ? g.round : g.round - 1;
           if (r >= 0) tc_wait(&bars.wfull[i], r & 1);
         }
       }
@@ -632,14 +637,17 @@ void plan_rows(TcParams& p, bool bwd) {
         if (used() + p.w_bytes <= budget) return;
     }
   }
-  // The ring holds at least one chunk's blocks twice over before a second
-  // row tile or hidden buffer is bought with it.
+  // The rings hold at least one chunk's blocks twice over before a second row
+  // tile or hidden buffer is bought with them; they share the slots by the
+  // blocks that a step takes from each.
   const int per_chunk = p.cd + (p.ko + 7) / 8;
   for (int more = 3; more >= 0; --more) {
     p.nh = 1 + (more >> 1 & 1), p.nx = 1 + (more & 1);
     p.slots = static_cast<int>(std::min<int64_t>(kMaxSlots, (budget - used()) / kBlockBytes));
-    if (p.slots >= std::min(2 * per_chunk, 6)) return;
+    if (p.slots >= std::min(2 * per_chunk, 6)) break;
   }
+  const int first = bwd ? per_chunk : p.cd, second = bwd ? p.cd : per_chunk - p.cd;
+  p.slots_f = std::min(p.slots - 1, std::max(1, (p.slots * first + (first + second) / 2) / (first + second)));
 }
 
 uint32_t rows_smem(const TcParams& p) {
