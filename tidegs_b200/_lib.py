@@ -350,7 +350,7 @@ KERNELS_PER_CALL = {
     # iota + the library radix sort and scan (their kernel counts depend on
     # the library version and are not counted here)
     "tgs_isect_depth_order": 1, "tgs_isect_sort_tiles": 0,
-    "tgs_layer_norm_fwd": 1, "tgs_layer_norm_bwd": 2, "tgs_ffn_fwd": 1, "tgs_ffn_bwd": 3,
+    "tgs_layer_norm_fwd": 1, "tgs_layer_norm_bwd": 2, "tgs_ffn_fwd": 1, "tgs_ffn_bwd": 2,
     "tgs_dropout": 1,
 }
 launch_counter = {"kernels": 0}

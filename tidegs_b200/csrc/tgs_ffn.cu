@@ -255,13 +255,10 @@ int64_t weights_floats(int64_t n, int d, int h, int o) {
 
 template <class T>
 int ffn_weights(const FfnParams& p, cudaStream_t s) {
-  int slices = 0;
-  if (p.n > 0) {
-    slices = ffn_slices(p.n, p.h);
-    if (int rc = p.d <= 64 && p.o <= 64 ? launch_weights<T, 8>(p, slices, s)
-                                        : launch_weights<T, 32>(p, slices, s))
-      return rc;
-  }
+  const int slices = ffn_slices(p.n, p.h);
+  if (int rc = p.d <= 64 && p.o <= 64 ? launch_weights<T, 8>(p, slices, s)
+                                      : launch_weights<T, 32>(p, slices, s))
+    return rc;
   const int64_t all = static_cast<int64_t>(p.h) * (2 * p.d + p.o);
   ffn_weights_sum_kernel<T><<<static_cast<unsigned>(ceil_div<int64_t>(all, kThreads)), kThreads, 0, s>>>(
       p.scratch, slices, p.d, p.h, p.o, static_cast<T*>(p.dwg), static_cast<T*>(p.dwu),
@@ -271,19 +268,11 @@ int ffn_weights(const FfnParams& p, cudaStream_t s) {
 }
 
 int ffn_backward_f32(const FfnParams& p, cudaStream_t s) {
-  if (p.y && p.n > 0) {
+  if (p.y) {
     if (int rc = p.d <= 64 ? launch_rows<float, true, 2>(p, s) : launch_rows<float, true, 8>(p, s))
       return rc;
   }
   return p.dwg ? ffn_weights<float>(p, s) : TGS_OK;
-}
-
-int ffn_backward_bf16(FfnParams p, cudaStream_t s) {
-  if (p.dwg) {
-    if (int rc = ffn_weights<__nv_bfloat16>(p, s)) return rc;
-  }
-  if (!p.y || p.n == 0) return TGS_OK;
-  return ffn_tc_backward(p, s);
 }
 
 int check_ffn(const TgsFfnArgs* a, const char* who) {
@@ -316,9 +305,9 @@ using namespace tgs;
 extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32_t o, int32_t dtype,
                                           int32_t backward) {
   if (n <= 0 || d <= 0 || h <= 0 || o <= 0) return 0;
-  if (!backward) return dtype == TGS_F32 ? 0 : ffn_tc_scratch_floats(n, d, h, o, false);
-  const int64_t weights = weights_floats(n, d, h, o);
-  return dtype == TGS_F32 ? weights : std::max(weights, ffn_tc_scratch_floats(n, d, h, o, true));
+  if (dtype != TGS_F32) return ffn_tc_scratch_floats(n, d, h, o, backward != 0);
+  if (!backward) return 0;
+  return weights_floats(n, d, h, o);
 }
 
 extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
@@ -347,6 +336,14 @@ extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {
   FfnParams p = ffn_params(a);
   p.dy = b->v_y, p.dy_stride = b->v_y_stride, p.y = b->v_x;
   p.dwg = b->v_w_gate, p.dwu = b->v_w_up, p.dwd = b->v_w_down;
-  return a.dtype == TGS_F32 ? ffn_backward_f32(p, as_stream(stream))
-                            : ffn_backward_bf16(p, as_stream(stream));
+  cudaStream_t s = as_stream(stream);
+  if (a.n == 0) {
+    if (!weights) return TGS_OK;
+    const size_t size = a.dtype == TGS_F32 ? 4 : 2, hd = size * a.h * a.d, ho = size * a.h * a.o;
+    TGS_CUDA(cudaMemsetAsync(p.dwg, 0, hd, s));
+    TGS_CUDA(cudaMemsetAsync(p.dwu, 0, hd, s));
+    TGS_CUDA(cudaMemsetAsync(p.dwd, 0, ho, s));
+    return TGS_OK;
+  }
+  return a.dtype == TGS_F32 ? ffn_backward_f32(p, s) : ffn_tc_backward(p, s);
 }

@@ -43,6 +43,7 @@ struct TcParams {
   CUtensorMap xmap, dymap;
   FfnParams f;
   const uint8_t* packed;  // laid-out weights (streaming)
+  float* partial;         // the weights' gradients by slice
   int64_t tiles;
   int cd, co, nc;  // operand blocks of D and O, chunks of H
   int kd, ko;      // 16-steps of D and O
@@ -51,12 +52,19 @@ struct TcParams {
   int resident, tma_x, tma_dy, vec_y;
   uint32_t tile_bytes, h_bytes, w_bytes;
   uint32_t tmem_cols;
+  // Block b takes chunks [cpc g, cpc g + cpc) of tiles s, s + slices, ... with
+  // g = b % groups and s = b / groups. With `split`, odd g are the blocks of
+  // dWd's gradient and even g those of the two others (for chunks g / 2).
+  int cpc, groups, slices, split;
 };
+
+// What a kernel computes: Y, dX, the weights' gradients, or the last two.
+enum : int { kFwd = 0, kDx = 1, kDw = 2, kDxDw = 3 };
 
 struct TcBars {
   uint64_t xfull[kMaxTiles], xempty[kMaxTiles];
   uint64_t gfull[2], gempty[2], hfull[kMaxHid], hempty[kMaxHid];
-  uint64_t yfull[2], yempty[2], done;
+  uint64_t yfull[2], yempty[2], done, accfull;
   uint64_t wfull[kMaxSlots], wempty[kMaxSlots];
   uint32_t tmem;
 };
@@ -66,11 +74,15 @@ struct TcBars {
 // of Wg and rows 64-127 those of Wu; then (after all chunks' blocks) Wd's
 // columns of the chunk as [16 ko][64]. Zeros beyond D, H and O.
 
+// `nj` chunks are laid out.
 __host__ __device__ __forceinline__ uint32_t wgu_offset(const TcParams& p, int j, int c) {
   return static_cast<uint32_t>(j * p.cd + c) * kBlockBytes;
 }
-__host__ __device__ __forceinline__ uint32_t wd_offset(const TcParams& p, int j, int b) {
-  return static_cast<uint32_t>(p.nc * p.cd) * kBlockBytes + j * p.ko * 2048 + b * kBlockBytes;
+__host__ __device__ __forceinline__ uint32_t wd_offset(const TcParams& p, int nj, int j, int b) {
+  return static_cast<uint32_t>(nj * p.cd) * kBlockBytes + j * p.ko * 2048 + b * kBlockBytes;
+}
+__host__ __device__ __forceinline__ uint32_t weight_bytes(const TcParams& p, int nj) {
+  return static_cast<uint32_t>(nj) * (p.cd * kBlockBytes + p.ko * 2048);
 }
 
 __device__ __forceinline__ uint4 load_unit(const __nv_bfloat16* src, int64_t at, int left,
@@ -88,14 +100,16 @@ __device__ __forceinline__ uint4 load_unit(const __nv_bfloat16* src, int64_t at,
   return u.q;
 }
 
-// 16-byte unit `e` of the laid-out weights: its value, and where it goes.
-__device__ __forceinline__ uint4 weight_unit(const TcParams& p, uint32_t e, uint32_t* offset) {
+// 16-byte unit `e` of the layout of chunks j0 to j0 + nj: its value, and
+// where it goes.
+__device__ __forceinline__ uint4 weight_unit(const TcParams& p, int j0, int nj, uint32_t e,
+                                             uint32_t* offset) {
   const FfnParams& f = p.f;
-  const uint32_t block = e >> 10, gu_blocks = p.nc * p.cd;
+  const uint32_t block = e >> 10, gu_blocks = nj * p.cd;
   if (block < gu_blocks) {
     const int j = block / p.cd, c = block - j * p.cd;
     const int row = (e >> 3) & 127, unit = e & 7;
-    const int hid = j * kChunk + (row & 63), col = c * kBlockCols + unit * 8;
+    const int hid = (j0 + j) * kChunk + (row & 63), col = c * kBlockCols + unit * 8;
     *offset = block * kBlockBytes + unit_offset(row, unit);
     if (hid >= f.h || col >= f.d) return make_uint4(0, 0, 0, 0);
     const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(row < 64 ? f.wg : f.wu);
@@ -104,7 +118,7 @@ __device__ __forceinline__ uint4 weight_unit(const TcParams& p, uint32_t e, uint
   }
   const uint32_t r = (e - (gu_blocks << 10)) >> 3;  // row over all chunks
   const int j = r / (16 * p.ko), row = r - j * 16 * p.ko, unit = e & 7;
-  const int col = j * kChunk + unit * 8;
+  const int col = (j0 + j) * kChunk + unit * 8;
   *offset = gu_blocks * kBlockBytes + j * p.ko * 2048 + unit_offset(row, unit);
   if (row >= f.o || col >= f.h) return make_uint4(0, 0, 0, 0);
   const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(f.wd);
@@ -114,9 +128,9 @@ __device__ __forceinline__ uint4 weight_unit(const TcParams& p, uint32_t e, uint
 
 __global__ void __launch_bounds__(256) ffn_pack_kernel(const TcParams p, uint8_t* dst) {
   const uint32_t e = blockIdx.x * 256 + threadIdx.x;
-  if (e >= p.w_bytes / 16) return;
+  if (e >= weight_bytes(p, p.nc) / 16) return;
   uint32_t at;
-  const uint4 v = weight_unit(p, e, &at);
+  const uint4 v = weight_unit(p, 0, p.nc, e, &at);
   *reinterpret_cast<uint4*>(dst + at) = v;
 }
 
@@ -195,39 +209,43 @@ __device__ __forceinline__ F2 sigmoid2(F2 g, bool& far) {
   return F2(r * b, r * a);
 }
 
-// 16 hidden values of a row, rounded and packed in pairs: act(G) U, or dG in
-// `p` and dU in `q`.
-template <bool kBwd, bool kEach>
-__device__ __forceinline__ bool activate(const float (&g)[16], const float (&u)[16],
-                                         const float (&dh)[16], uint32_t (&p)[8],
-                                         uint32_t (&q)[8]) {
+// kW hidden values of a row, rounded and packed in pairs: h = act(G) U in the
+// forward; dG, dU and (for the weights' gradients) h in the backward.
+template <int kMode, bool kEach, int kW>
+__device__ __forceinline__ bool activate(const float (&g)[kW], const float (&u)[kW],
+                                         const float (&dh)[kW], uint32_t (&h)[kW / 2],
+                                         uint32_t (&dg)[kW / 2], uint32_t (&du)[kW / 2]) {
   bool far = false;
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
+  for (int i = 0; i < kW; i += 2) {
     const F2 g2(g[i], g[i + 1]), u2(u[i], u[i + 1]), s2 = sigmoid2<kEach>(g2, far);
     const F2 act = g2 * s2;
     float a, b;
-    if constexpr (kBwd) {
+    if constexpr (kMode != kDx) {
+      (act * u2).get(a, b);
+      h[i / 2] = pack_bf16(a, b);
+    }
+    if constexpr (kMode != kFwd) {
       const F2 d2(dh[i], dh[i + 1]);
       // silu'(g) = s + act (1 - s)
       const F2 slope = fma2(act, fma2(s2, F2(-1.f, -1.f), F2(1.f, 1.f)), s2);
       (d2 * u2 * slope).get(a, b);
-      p[i / 2] = pack_bf16(a, b);
+      dg[i / 2] = pack_bf16(a, b);
       (d2 * act).get(a, b);
-      q[i / 2] = pack_bf16(a, b);
-    } else {
-      (act * u2).get(a, b);
-      p[i / 2] = pack_bf16(a, b);
+      du[i / 2] = pack_bf16(a, b);
     }
   }
   return far;
 }
 
-// Puts them into units 2 g16 and 2 g16 + 1 of a block's row.
-__device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint32_t g16,
-                                              const uint32_t (&v)[8]) {
-  st_shared16(block + unit_offset(row, 2 * g16), make_uint4(v[0], v[1], v[2], v[3]));
-  st_shared16(block + unit_offset(row, 2 * g16 + 1), make_uint4(v[4], v[5], v[6], v[7]));
+// Puts kW values into a block's row, from column kW g on.
+template <int kN>
+__device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint32_t g,
+                                              const uint32_t (&v)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN / 4; ++i)
+    st_shared16(block + unit_offset(row, g * (kN / 4) + i),
+                make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
 }
 
 // A row tile -> operand blocks, by threads: for matrices that no tensor map
@@ -256,7 +274,7 @@ __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, in
   const int64_t row = tile * kTile + lane_row;
   for (int c = 0; c < out; c += 16) {
     float v[16];
-    tmem_ld16(acc + c, v);
+    tmem_ld(acc + c, v);
     tmem_wait_ld(v);
     __nv_bfloat16* dst = y + row * out + c;
     if (row >= p.f.n) {
@@ -281,9 +299,30 @@ __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, in
   }
 }
 
-// --- rows: Y, or dX --------------------------------------------------------------
-template <bool kBwd>
-__global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid_constant__ TcParams p) {
+// This block's sum of one weight gradient's chunk, out of its accumulators.
+__device__ __forceinline__ void store_partial(uint32_t acc, float* dst, int cols, bool on) {
+  for (int c = 0; c < cols; c += 16) {
+    float v[16];
+    tmem_ld(acc + c, v);
+    tmem_wait_ld(v);
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(dst + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
+    __syncwarp();
+  }
+}
+
+// Floats of a chunk's gradients in `partial`: [128][16 kd] rows of dWg and
+// dWu, then [64][16 ko] columns of dWd.
+__host__ __device__ __forceinline__ int chunk_floats(const TcParams& p) {
+  return 16 * (128 * p.kd + 64 * p.ko);
+}
+
+// --- the kernel --------------------------------------------------------------------
+template <int kMode>
+__global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_constant__ TcParams p) {
   extern __shared__ uint8_t raw[];
   __shared__ TcBars bars;
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
@@ -292,8 +331,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   const uint32_t ws = hs + p.nh * p.h_bytes;            // weights, or the ring
   // from lane 0, so that the compiler sees the roles' branches as uniform
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int mine = static_cast<int>((p.tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
-  const int steps = mine * p.nc;  // n <= 2^31 and H <= 4096: below 2^30 of them
+  constexpr bool kBwd = kMode != kFwd, kHasDw = kMode >= kDw, kRows = kMode != kDw;
+  const int group_id = kHasDw ? blockIdx.x % p.groups : 0;
+  const int slice = kHasDw ? blockIdx.x / p.groups : blockIdx.x;
+  const bool want_gu = !kHasDw || !p.split || !(group_id & 1);  // dWg and dWu
+  const bool want_d = !kHasDw || !p.split || (group_id & 1);    // dWd
+  const int j0 = (p.split ? group_id >> 1 : group_id) * p.cpc;
+  const int nj = min(p.cpc, p.nc - j0);
+  const int mine = static_cast<int>((p.tiles - slice + p.slices - 1) / p.slices);
+  const int steps = mine * nj;  // n <= 2^31 and H <= 4096: below 2^30 of them
+  // where chunk j's weights are: of this block's chunks, or of all
+  const int laid = p.resident ? p.cpc : p.nc, jw = p.resident ? 0 : j0;
   const int wblocks = (p.ko + 7) / 8;  // blocks of Wd per chunk
   constexpr uint32_t kGCols = kBwd ? 192 : 128;
   Waits wait{p.f.err};
@@ -308,7 +356,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         mbar_init(&bars.yfull[i], 1), mbar_init(&bars.yempty[i], kLoad / 32);
       }
       for (int i = 0; i < kMaxHid; ++i) mbar_init(&bars.hfull[i], kEpi / 64), mbar_init(&bars.hempty[i], 1);
-      mbar_init(&bars.done, 2);
+      mbar_init(&bars.done, 2), mbar_init(&bars.accfull, 1);
       for (int i = 0; i < kMaxSlots; ++i) mbar_init(&bars.wfull[i], 1), mbar_init(&bars.wempty[i], 1);
       fence_mbar_init();
     }
@@ -316,7 +364,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   if (p.resident) {
     for (uint32_t e = threadIdx.x; e < p.w_bytes / 16; e += kTcThreads) {
       uint32_t at;
-      const uint4 v = weight_unit(p, e, &at);
+      const uint4 v = weight_unit(p, j0, p.cpc, e, &at);
       st_shared16(ws + at, v);
     }
     fence_proxy_async_smem();
@@ -326,36 +374,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
   const uint32_t yacc = tmem + p.nb * kGCols;
+  const uint32_t wacc = yacc + p.ny * p.ycols;  // gradients: per chunk gu_cols + d_cols
+  const uint32_t gu_cols = want_gu ? 16 * p.kd : 0, d_cols = want_d ? 16 * p.ko : 0;
+  const uint32_t dg_at = kHasDw && want_d ? kBlockBytes : 0;  // hidden buffer: h, dG, dU
 
-  // Step `it` (tile it / nc, chunk it % nc) signals on the barriers it % 2, and
+  // Step `it` (tile it / nj, chunk it % nj) signals on the barriers it % 2, and
   // it % hm for the hidden buffers, a tile t on those of t % 2, whether or not
   // there are two buffers: a wait then never meets a barrier that is two phases
   // from the awaited one, which it could not tell from it.
   const int hm = max(p.nh, 2);
   if (warp < kWarpF) {
     // Activation: group warp / 8 takes the steps of its parity; this thread's
-    // row of the tile, and the 16-column granules half, half + 2 of the chunk.
+    // row of the tile, and every second granule of kW columns of the chunk.
     const uint32_t row = (warp & 3) * 32 + lane;
     const int group = warp >> 3, half = warp >> 2 & 1;
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;  // lane 32 (warp % 4)
     int j = group;
     int hb = group, hphase = 0;
     for (int it = group; it < steps; it += 2, j += 2, hb += 2) {
-      while (j >= p.nc) j -= p.nc;
+      while (j >= nj) j -= nj;
       if (hb >= hm) hb -= hm, ++hphase;
       wait(&bars.gfull[group], it >> 1);
       tc_fence_after();
       const uint32_t acc = tmem + (p.nb == 2 ? group : 0) * kGCols + quarter;
       const uint32_t hbuf = hs + (p.nh > 1 ? hb : 0) * p.h_bytes;
-      const int grans = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
+      // whole 16-steps of the chunk's hidden values
+      const int cols = (min(kChunk, p.f.h - (j0 + j) * kChunk) + 15) & ~15;
       constexpr int kParts = kBwd ? 3 : 2;  // G, U, dH
+      constexpr int kW = kHasDw ? 8 : 16;   // what the registers hold
+      constexpr int kTurns = kChunk / kW / 2;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < kTurns; ++i) {
         const int q = half + 2 * i;
-        float v[kParts][16];
-        if (q < grans) {
+        float v[kParts][kW];
+        if (q * kW < cols) {
 #pragma unroll
-          for (int k = 0; k < kParts; ++k) tmem_ld16(acc + 64 * k + 16 * q, v[k]);
+          for (int k = 0; k < kParts; ++k) tmem_ld(acc + 64 * k + kW * q, v[k]);
         }
         if (i == 0) {  // meanwhile: the step that last used the hidden buffer
           if (p.nh > 1) {
@@ -364,20 +418,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
             wait(&bars.hempty[(it - 1) & 1], (it - 1) >> 1);
           }
         }
-        if (q < grans) {
+        if (q * kW < cols) {
 #pragma unroll
           for (int k = 0; k < kParts; ++k) tmem_wait_ld(v[k]);
         }
-        if (i == 1) {
+        if (i == kTurns - 1) {
           tc_fence_before();
           warp_arrive(&bars.gempty[group], lane);  // the accumulators have been read
         }
-        if (q < grans) {
-          uint32_t h0[8], h1[8];
-          if (activate<kBwd, kBwd>(v[0], v[1], v[kParts - 1], h0, h1))
-            activate<kBwd, true>(v[0], v[1], v[kParts - 1], h0, h1);
-          store_granule(hbuf, row, q, h0);
-          if constexpr (kBwd) store_granule(hbuf + kBlockBytes, row, q, h1);
+        if (q * kW < cols) {
+          uint32_t h[kW / 2], dg[kW / 2], du[kW / 2];
+          if (activate<kMode, kBwd>(v[0], v[1], v[kParts - 1], h, dg, du))
+            activate<kMode, true>(v[0], v[1], v[kParts - 1], h, dg, du);
+          if (kMode == kFwd || (kHasDw && want_d)) store_granule(hbuf, row, q, h);
+          if (kBwd && want_gu) {
+            store_granule(hbuf + dg_at, row, q, dg);
+            store_granule(hbuf + dg_at + kBlockBytes, row, q, du);
+          }
         }
       }
       fence_proxy_async_smem();
@@ -415,7 +472,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         }
         if constexpr (kBwd) {
           for (int b8 = 0; b8 < wblocks; ++b8) {
-            const uint32_t w = acquire(wd_offset(p, j, b8));
+            const uint32_t w = acquire(wd_offset(p, laid, j, b8));
             for (int c = 0; c < 2 && 2 * b8 + c < p.co; ++c)
               tc_mma_steps<4>(acc + 128, desc_k(dy + (2 * b8 + c) * kBlockBytes), kStepK,
                               desc_mn(w + c * 64 * 128, kBlockBytes), kStepMn,
@@ -424,37 +481,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
           }
         }
         tc_commit(&bars.gfull[it & 1]);
-        if (++j == p.nc) {
-          tc_commit(&bars.xempty[xb]);
+        if (++j == nj) {
+          if (!kHasDw) tc_commit(&bars.xempty[xb]);
           j = 0;
           if (++xb == p.nx) xb = 0, ++xround;
         }
       }
     } else {
-      int j = 0, t = 0, hb = 0, hphase = 0;
+      int j = 0, t = 0, hb = 0, hphase = 0, xb = 0;
       for (int it = 0; it < steps; ++it) {
         wait(&bars.hfull[hb], hphase);
-        if (j == 0 && t >= p.ny) wait(&bars.yempty[(t - p.ny) & 1], (t - p.ny) >> 1);
+        if (kRows && j == 0 && t >= p.ny) wait(&bars.yempty[(t - p.ny) & 1], (t - p.ny) >> 1);
         tc_fence_after();
         const uint32_t y = yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols;
         const uint32_t h = hs + (p.nh > 1 ? hb : 0) * p.h_bytes;
-        const int ks = (min(kChunk, p.f.h - j * kChunk) + 15) >> 4;
-        if constexpr (kBwd) {
+        const int ks = (min(kChunk, p.f.h - (j0 + j) * kChunk) + 15) >> 4;
+        if constexpr (kHasDw) {
+          // Operands with rows as K: [dG | dU]^T X as one product of 128 hidden
+          // columns; of [h | dG]^T dY only the first 64 are read.
+          const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
+          const uint32_t acc = wacc + j * (gu_cols + d_cols);
+          if (want_gu)
+            tc_mma_steps<8>(acc, desc_mn(h + dg_at, kBlockBytes), kStepMn, desc_mn(x, kBlockBytes),
+                            kStepMn, tc_idesc(gu_cols, true, true), 8, t > 0);
+          if (want_d)
+            tc_mma_steps<8>(acc + gu_cols, desc_mn(h, kBlockBytes), kStepMn,
+                            desc_mn(dy, kBlockBytes), kStepMn, tc_idesc(d_cols, true, true), 8,
+                            t > 0);
+        }
+        if constexpr (kBwd && kRows) {
           // dG Wg + dU Wu: the blocks' columns are N, their rows K
           const int wide = p.resident ? p.cd : 1;  // neighbouring blocks as one product
           for (int c = 0; c < p.cd; c += wide) {
             const uint32_t w = acquire(wgu_offset(p, j, c));
             const uint32_t id = tc_idesc(min(64 * wide, 16 * p.kd - 64 * c), false, true);
-            tc_mma_steps<4>(y + 64 * c, desc_k(h), kStepK, desc_mn(w, kBlockBytes), kStepMn, id,
-                            ks, j > 0);
-            tc_mma_steps<4>(y + 64 * c, desc_k(h + kBlockBytes), kStepK,
+            tc_mma_steps<4>(y + 64 * c, desc_k(h + dg_at), kStepK, desc_mn(w, kBlockBytes), kStepMn,
+                            id, ks, j > 0);
+            tc_mma_steps<4>(y + 64 * c, desc_k(h + dg_at + kBlockBytes), kStepK,
                             desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
             release();
           }
-        } else {
+        }
+        if constexpr (!kBwd) {
           const int wide = p.resident ? wblocks : 1;
           for (int b8 = 0; b8 < wblocks; b8 += wide) {
-            const uint32_t w = acquire(wd_offset(p, j, b8));
+            const uint32_t w = acquire(wd_offset(p, laid, j, b8));
             tc_mma_steps<4>(y + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
                             tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
                             j > 0);
@@ -463,11 +534,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         }
         tc_commit(&bars.hempty[hb]);
         if (++hb == hm) hb = 0, ++hphase;
-        if (++j == p.nc) {
-          tc_commit(&bars.yfull[t & 1]);
+        if (++j == nj) {
+          if (kRows) tc_commit(&bars.yfull[t & 1]);
+          if (kHasDw) tc_commit(&bars.xempty[xb]);
+          if (++xb == p.nx) xb = 0;
           j = 0, ++t;
         }
       }
+      if (kHasDw) tc_commit(&bars.accfull);
     }
     tc_commit(&bars.done);
     if (!tc_wait(&bars.done, 0))
@@ -486,11 +560,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         if (++r.slot == r.end) r.slot = r.begin, ++r.round;
       };
       auto put_gu = [&](Ring& r, int j) {
-        for (int c = 0; c < p.cd; ++c) put(r, wgu_offset(p, j, c), kBlockBytes);
+        for (int c = 0; c < p.cd; ++c) put(r, wgu_offset(p, jw + j, c), kBlockBytes);
       };
       auto put_d = [&](Ring& r, int j) {
         for (int b8 = 0; b8 < wblocks; ++b8)
-          put(r, wd_offset(p, j, b8), min(8, p.ko - 8 * b8) * 2048);
+          put(r, wd_offset(p, laid, jw + j, b8), min(8, p.ko - 8 * b8) * 2048);
       };
       // F0, F1 S0, F2 S1, ...: no first products wait for blocks that only come
       // after those of a second product that waits for them.
@@ -499,15 +573,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         if (it + 1 < steps) {
           put_gu(first, j1);
           if (kBwd) put_d(first, j1);
-          if (++j1 == p.nc) j1 = 0;
+          if (++j1 == nj) j1 = 0;
         }
-        if (it >= 0) {
+        if (kRows && it >= 0) {
           if (kBwd) {
             put_gu(second, j);
           } else {
             put_d(second, j);
           }
-          if (++j == p.nc) j = 0;
+          if (++j == nj) j = 0;
         }
         if (!wait.ok) break;
       }
@@ -525,7 +599,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
       for (int t = 0; t < mine && wait.ok; ++t) {
         if (round > 0) wait(&bars.xempty[xb], round - 1);
         if (!wait.ok) break;
-        const int64_t r0 = (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile;
+        const int64_t r0 = (slice + static_cast<int64_t>(t) * p.slices) * kTile;
         const uint32_t dst = xs + xb * p.tile_bytes;
         const int xblocks = p.tma_x ? p.cd : 0, yblocks = kBwd && p.tma_dy ? p.co : 0;
         mbar_arrive_expect_tx(&bars.xfull[xb], (xblocks + yblocks) * kBlockBytes);
@@ -549,7 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
     const int tid = threadIdx.x - kEpi - 128;
     const int out = kBwd ? p.f.d : p.f.o;
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;
-    auto row_of = [&](int t) { return (blockIdx.x + static_cast<int64_t>(t) * gridDim.x) * kTile; };
+    auto row_of = [&](int t) { return (slice + static_cast<int64_t>(t) * p.slices) * kTile; };
     int xb = 0, round = 0;
     // Loads run nx tiles ahead of the output: the buffer that a load waits for
     // is then never one whose tile waits for this output.
@@ -569,7 +643,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         if (++xb == p.nx) xb = 0, ++round;
       }
       const int done = t - ahead;
-      if (done >= 0) {
+      if (kRows && done >= 0) {
         wait(&bars.yfull[done & 1], done >> 1);
         tc_fence_after();
         store_output(p, yacc + (p.ny == 2 ? done & 1 : 0) * p.ycols + quarter,
@@ -578,6 +652,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
         warp_arrive(&bars.yempty[done & 1], lane);
       }
     }
+    if constexpr (kHasDw) {
+      // the whole sweep's end: one wait's limit for every 4096 steps
+      for (int k = 0; k < steps / 4096 && !tc_wait(&bars.accfull, 0); ++k) {
+      }
+      wait(&bars.accfull, 0);
+      tc_fence_after();
+      const int row = (warp & 3) * 32 + lane;
+      for (int j = 0; j < nj; ++j) {
+        float* dst = p.partial + (static_cast<int64_t>(slice) * p.nc + j0 + j) * chunk_floats(p);
+        const uint32_t acc = wacc + j * (gu_cols + d_cols) + quarter;
+        const bool on = (row & 63) < p.f.h - (j0 + j) * kChunk;
+        if (want_gu) store_partial(acc, dst + row * 16 * p.kd, gu_cols, on);
+        if (want_d && row < 64)
+          store_partial(acc + gu_cols, dst + 128 * 16 * p.kd + row * 16 * p.ko, d_cols, on);
+      }
+      tc_fence_before();
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -585,6 +676,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_rows_kernel(const __grid
   if (warp == kWarpF) {
     tc_fence_after();
     tmem_free(tmem, p.tmem_cols);
+  }
+}
+
+// The slices' sums in a fixed order, rounded into the weights' layouts: 128
+// neighbouring floats a block, the slices dealt to its eight warps.
+__global__ void __launch_bounds__(256) ffn_tc_sum_kernel(const TcParams p) {
+  __shared__ float4 part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int floats = chunk_floats(p);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 128 + 4 * lane;
+  const int64_t stride = static_cast<int64_t>(p.nc) * floats;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = warp; s < p.slices; s += 8) {
+    const float4 v = *reinterpret_cast<const float4*>(p.partial + s * stride + at);
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  part[warp][lane] = sum;
+  __syncthreads();
+  if (warp > 0) return;
+  for (int w = 1; w < 8; ++w) {
+    const float4 v = part[w][lane];
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  const int j = static_cast<int>(at / floats), e = static_cast<int>(at - static_cast<int64_t>(j) * floats);
+  const FfnParams& f = p.f;
+  const int gu = 128 * 16 * p.kd;
+  const bool up = e < gu;
+  const int width = up ? 16 * p.kd : 16 * p.ko;
+  const int row = (up ? e : e - gu) / width, col = (up ? e : e - gu) - row * width;
+  const int hid = j * kChunk + (row & 63);
+  if (hid >= f.h) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat16 r = __float2bfloat16_rn(v[i]);
+    if (up) {
+      if (col + i < f.d)
+        static_cast<__nv_bfloat16*>(row < 64 ? f.dwg : f.dwu)[static_cast<int64_t>(hid) * f.d + col + i] = r;
+    } else if (col + i < f.o) {
+      static_cast<__nv_bfloat16*>(f.dwd)[static_cast<int64_t>(col + i) * f.h + hid] = r;
+    }
   }
 }
 
@@ -600,7 +733,7 @@ TcParams tc_params(const FfnParams& f) {
   p.kd = ceil_div(f.d, 16), p.ko = ceil_div(f.o, 16);
   p.cd = ceil_div(f.d, 64), p.co = ceil_div(f.o, 64), p.nc = ceil_div(f.h, kChunk);
   p.tiles = ceil_div<int64_t>(f.n, kTile);
-  p.w_bytes = static_cast<uint32_t>(p.nc) * (p.cd * kBlockBytes + p.ko * 2048);
+  p.cpc = p.nc, p.groups = 1;
   return p;
 }
 
@@ -615,7 +748,7 @@ int make_maps(TcParams& p, bool bwd) {
   return p.tma_dy ? make_row_map(&p.dymap, f.dy, f.n, f.o, f.dy_stride) : TGS_OK;
 }
 
-// Buffers of the rows kernel. Shared memory goes first to the weights (as a
+// Buffers for Y or dX. Shared memory goes first to the weights (as a
 // whole where two row tiles and two hidden buffers fit beside them), then to
 // whatever keeps the most work in flight.
 void plan_rows(TcParams& p, bool bwd) {
@@ -626,6 +759,8 @@ void plan_rows(TcParams& p, bool bwd) {
   p.ny = p.nb * g + 2 * out <= 512 ? 2 : 1;
   p.ycols = out;
   p.tmem_cols = pow2_cols(p.nb * g + p.ny * out);
+  p.w_bytes = weight_bytes(p, p.nc);
+  p.slices = static_cast<int>(std::min<int64_t>(p.tiles, sm_count()));
   const int64_t budget = kSmemBudget;
   auto used = [&] { return static_cast<int64_t>(p.nx) * p.tile_bytes + p.nh * p.h_bytes; };
   p.nx = 2, p.nh = 2, p.slots = 1;
@@ -650,32 +785,96 @@ void plan_rows(TcParams& p, bool bwd) {
   p.slots_f = std::min(p.slots - 1, std::max(1, (p.slots * first + (first + second) / 2) / (first + second)));
 }
 
-uint32_t rows_smem(const TcParams& p) {
+// Buffers for the weights' gradients, whose accumulators stay in tensor memory
+// over all of a block's tiles: as many chunks per block as fit there. With
+// `dx`, whether all of them fit beside dX's, so that one kernel gives both.
+bool plan_weights(TcParams& p, bool dx) {
+  const int gu = 16 * p.kd, d = 16 * p.ko;
+  p.tile_bytes = (p.cd + p.co) * kBlockBytes;
+  p.nb = 1, p.ny = dx ? 1 : 0, p.ycols = dx ? gu : 0;
+  p.split = 192 + gu + d > 512;
+  if (dx && (p.split || 192 + gu + p.nc * (gu + d) > 512)) return false;
+  const int cols = p.split ? std::max(gu, d) : gu + d;
+  p.cpc = std::min(p.nc, (512 - 192 - p.ycols) / cols);
+  p.groups = ceil_div(p.nc, p.cpc);
+  p.cpc = ceil_div(p.nc, p.groups);
+  if (!dx && 2 * 192 + p.cpc * cols <= 512) p.nb = 2;
+  p.tmem_cols = pow2_cols(p.nb * 192 + p.ycols + p.cpc * cols);
+  if (p.split) p.groups *= 2;
+  p.slices = static_cast<int>(std::min<int64_t>(p.tiles, std::max(1, sm_count() / p.groups)));
+  p.h_bytes = (p.split ? 2 : 3) * kBlockBytes;
+  p.w_bytes = weight_bytes(p, p.cpc);
+  const int64_t budget = kSmemBudget;
+  auto used = [&] { return static_cast<int64_t>(p.nx) * p.tile_bytes + p.nh * p.h_bytes; };
+  const int tries[][2] = {{3, 2}, {2, 2}, {2, 1}, {1, 2}, {1, 1}};
+  p.resident = 1, p.slots = p.slots_f = 0;
+  for (const auto& t : tries) {
+    p.nx = t[0], p.nh = t[1];
+    if (used() + p.w_bytes <= budget) return true;
+  }
+  if (dx) return false;
+  p.resident = 0;
+  for (const auto& t : tries) {
+    p.nx = t[0], p.nh = t[1];
+    p.slots = static_cast<int>(std::min<int64_t>(kMaxSlots, (budget - used()) / kBlockBytes));
+    if (p.slots >= 3) break;
+  }
+  p.slots_f = p.slots;
+  return true;
+}
+
+uint32_t tc_smem(const TcParams& p) {
   return p.nx * p.tile_bytes + p.nh * p.h_bytes +
          (p.resident ? p.w_bytes : p.slots * kBlockBytes) + 1024;
 }
 
-template <bool kBwd>
-int launch_tc_rows(TcParams p, cudaStream_t s) {
-  plan_rows(p, kBwd);
-  const int smem = static_cast<int>(rows_smem(p));
-  // Before the tensor maps: this binds the thread's context, which a thread of
-  // autograd's may not have yet and the encoder needs.
-  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_rows_kernel<kBwd>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  if (int rc = make_maps(p, kBwd)) return rc;
-  const int out = kBwd ? p.f.d : p.f.o;
-  p.vec_y = out % 8 == 0 && aligned16(p.f.y);
-  if (!p.resident) {
-    uint8_t* packed = reinterpret_cast<uint8_t*>(p.f.scratch);
-    p.packed = packed;
-    ffn_pack_kernel<<<ceil_div<uint32_t>(p.w_bytes / 16, 256), 256, 0, s>>>(p, packed);
-    TGS_LAUNCH_CHECK();
-  }
-  const int grid = static_cast<int>(std::min<int64_t>(p.tiles, sm_count()));
-  ffn_tc_rows_kernel<kBwd><<<grid, kTcThreads, smem, s>>>(p);
+int pack_weights(const TcParams& p, uint8_t* dst, cudaStream_t s) {
+  ffn_pack_kernel<<<ceil_div<uint32_t>(weight_bytes(p, p.nc) / 16, 256), 256, 0, s>>>(p, dst);
   TGS_LAUNCH_CHECK();
   return TGS_OK;
+}
+
+template <int kMode>
+int launch_tc(TcParams p, cudaStream_t s) {
+  const int smem = static_cast<int>(tc_smem(p));
+  // Before the tensor maps: this binds the thread's context, which a thread of
+  // autograd's may not have yet and the encoder needs.
+  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                smem));
+  if (int rc = make_maps(p, kMode != kFwd)) return rc;
+  const int out = kMode == kFwd ? p.f.o : p.f.d;
+  p.vec_y = out % 8 == 0 && aligned16(p.f.y);
+  ffn_tc_kernel<kMode><<<p.groups * p.slices, kTcThreads, smem, s>>>(p);
+  TGS_LAUNCH_CHECK();
+  return TGS_OK;
+}
+
+// How a backward call runs: as one kernel (`both`), or as one for dX and one
+// for the weights' gradients; the laid-out weights follow the partial sums.
+struct BwdPlan {
+  TcParams rows, weights;
+  bool both;
+  int64_t partial, floats;
+};
+
+BwdPlan plan_backward(const FfnParams& f, bool dx, bool dw) {
+  BwdPlan b{};
+  b.rows = b.weights = tc_params(f);
+  b.both = dx && dw && plan_weights(b.weights, true);
+  bool packed = false;
+  if (dw && !b.both) {
+    b.weights = tc_params(f);
+    plan_weights(b.weights, false);
+    packed |= !b.weights.resident;
+  }
+  if (dx && !b.both) {
+    plan_rows(b.rows, true);
+    packed |= !b.rows.resident;
+  }
+  if (dw)
+    b.partial = static_cast<int64_t>(b.weights.slices) * b.weights.nc * chunk_floats(b.weights);
+  b.floats = b.partial + (packed ? weight_bytes(b.rows, b.rows.nc) / 4 : 0);
+  return b;
 }
 
 }  // namespace
@@ -705,19 +904,46 @@ int make_row_map(CUtensorMap* map, const void* base, int64_t rows, int cols, int
 }
 
 int ffn_tc_forward(const FfnParams& f, cudaStream_t s) {
-  return launch_tc_rows<false>(tc_params(f), s);
+  TcParams p = tc_params(f);
+  plan_rows(p, false);
+  if (!p.resident) {
+    p.packed = reinterpret_cast<const uint8_t*>(f.scratch);
+    if (int rc = pack_weights(p, reinterpret_cast<uint8_t*>(f.scratch), s)) return rc;
+  }
+  return launch_tc<kFwd>(p, s);
 }
 
 int64_t ffn_tc_scratch_floats(int64_t n, int d, int h, int o, bool backward) {
   FfnParams f{};
   f.n = n, f.d = d, f.h = h, f.o = o;
-  TcParams p = tc_params(f);
-  plan_rows(p, backward);
-  return p.resident ? 0 : p.w_bytes / 4;
+  if (!backward) {
+    TcParams p = tc_params(f);
+    plan_rows(p, false);
+    return p.resident ? 0 : weight_bytes(p, p.nc) / 4;
+  }
+  // whichever gradients are asked for
+  return std::max(plan_backward(f, true, true).floats,
+                  std::max(plan_backward(f, true, false).floats, plan_backward(f, false, true).floats));
 }
 
 int ffn_tc_backward(const FfnParams& f, cudaStream_t s) {
-  return launch_tc_rows<true>(tc_params(f), s);
+  const bool dx = f.y != nullptr, dw = f.dwg != nullptr;
+  BwdPlan b = plan_backward(f, dx, dw);
+  if (b.floats > b.partial) {
+    uint8_t* packed = reinterpret_cast<uint8_t*>(f.scratch + b.partial);
+    b.rows.packed = b.weights.packed = packed;
+    if (int rc = pack_weights(b.rows, packed, s)) return rc;
+  }
+  b.weights.partial = f.scratch;
+  if (dx && !b.both) {
+    if (int rc = launch_tc<kDx>(b.rows, s)) return rc;
+  }
+  if (!dw) return TGS_OK;
+  if (int rc = b.both ? launch_tc<kDxDw>(b.weights, s) : launch_tc<kDw>(b.weights, s)) return rc;
+  ffn_tc_sum_kernel<<<static_cast<unsigned>(b.weights.nc * (chunk_floats(b.weights) / 128)), 256, 0, s>>>(
+      b.weights);
+  TGS_LAUNCH_CHECK();
+  return TGS_OK;
 }
 
 }  // namespace tgs

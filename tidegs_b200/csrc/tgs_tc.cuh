@@ -136,10 +136,17 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols));
 }
 
-// 16 columns of this warp's 32 lanes: lane l of the quarter holds row l. The
-// registers hold the values only after tmem_wait_ld, which is given them so
-// that no use of them can move ahead of it.
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+// 8 or 16 columns of this warp's 32 lanes: lane l of the quarter holds row l.
+// The registers hold the values only after tmem_wait_ld, which is given them
+// so that no use of them can move ahead of it.
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
       "%12, %13, %14, %15}, [%16];"
@@ -147,6 +154,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
         "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
         "=f"(v[14]), "=f"(v[15])
       : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]),
+                 "+f"(v[7])
+               :
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld(float (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
