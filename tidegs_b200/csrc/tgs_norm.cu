@@ -8,8 +8,10 @@
 // from the row it reads anyway instead of reading them back. All sums are in
 // 32 bits; only y and the gradients are rounded to the tensors' types, once.
 //
-// Bound: HBM. A group of `lanes` threads (a power of two, at most a warp)
-// holds one row of at most 1024 values; wider rows take a whole block.
+// Bound: HBM. A group of `lanes` threads holds kU rows at a time, as they were
+// loaded (16-byte vectors, or single values where width or alignment forbid
+// them), so that enough bytes are on their way: a warp or a part of one per
+// row, or the whole block for wide rows, where the kU rows share the barriers.
 #include "tgs_common.cuh"
 #include "tgs_vec.cuh"
 
@@ -18,24 +20,32 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxC = 8192;
+constexpr int kNormBlocksPerSm = 8;
 
-// Sum over the group of threads that holds a row: `lanes` neighbours within a
-// warp, or the whole block (kBlock) through shared memory.
-template <bool kBlock>
-__device__ __forceinline__ float group_sum(float v, int lanes, float* red) {
+// Sums of kU values over the group of threads that holds a row: `lanes`
+// neighbours within a warp, or the whole block (kBlock) through shared memory.
+template <bool kBlock, int kU>
+__device__ __forceinline__ void group_sum(float (&v)[kU], int lanes, float (*red)[kU]) {
   if constexpr (kBlock) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    __syncthreads();  // the previous sum has been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.f;
+    for (int off = 16; off > 0; off >>= 1)
 #pragma unroll
-    for (int w = 0; w < kNormThreads / 32; ++w) t += red[w];
-    return t;
+      for (int k = 0; k < kU; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+    __syncthreads();  // the previous sums have been read
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < kU; ++k) red[threadIdx.x >> 5][k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kU; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kNormThreads / 32; ++w) v[k] += red[w][k];
+    }
   } else {
-    for (int off = lanes >> 1; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
+    for (int off = lanes >> 1; off > 0; off >>= 1)
+#pragma unroll
+      for (int k = 0; k < kU; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
   }
 }
 
@@ -51,15 +61,63 @@ struct NormParams {
   float eps;
 };
 
-// kVec values per load, kNv loads per thread and row: thread t of a group
-// holds columns (t + lanes j) kVec + i.
-template <class T, int kVec, int kNv, bool kBlock>
+// kVec values per load, kNv loads per thread and row, kU rows at a time:
+// thread t of a group holds columns (t + lanes j) kVec + i.
+template <class T, int kVec, int kNv, int kU, bool kBlock>
+struct NormRows {
+  Packed<T, kVec> x[kU][kNv];
+
+  __device__ __forceinline__ void load(const T* src, int64_t stride, int64_t r0, int64_t n,
+                                       int groups, int t, int lanes, int c) {
+#pragma unroll
+    for (int k = 0; k < kU; ++k) {
+      const int64_t r = r0 + static_cast<int64_t>(k) * groups;
+#pragma unroll
+      for (int j = 0; j < kNv; ++j) {
+        const int col = (t + lanes * j) * kVec;
+        x[k][j].load(src + r * stride + col, r < n && col < c);
+      }
+    }
+  }
+
+  // Means, and 1 / sqrt(variance + eps), of the rows.
+  __device__ __forceinline__ void stats(float (&mean)[kU], float (&rstd)[kU], int t, int lanes, int c,
+                                        float inv_c, float eps, float (*red)[kU]) {
+#pragma unroll
+    for (int k = 0; k < kU; ++k) {
+      mean[k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kNv; ++j)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) mean[k] += x[k][j].get(i);
+    }
+    group_sum<kBlock>(mean, lanes, red);
+#pragma unroll
+    for (int k = 0; k < kU; ++k) {
+      mean[k] *= inv_c;
+      rstd[k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kNv; ++j) {
+        const bool in = (t + lanes * j) * kVec < c;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const float d = in ? x[k][j].get(i) - mean[k] : 0.f;
+          rstd[k] += d * d;
+        }
+      }
+    }
+    group_sum<kBlock>(rstd, lanes, red);
+#pragma unroll
+    for (int k = 0; k < kU; ++k) rstd[k] = rsqrtf(rstd[k] * inv_c + eps);
+  }
+};
+
+template <class T, int kVec, int kNv, int kU, bool kBlock>
 __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(const NormParams p) {
-  __shared__ float red[kNormThreads / 32];
+  __shared__ float red[kNormThreads / 32][kU];
   const int lanes = p.lanes, c = p.c;
   const int t = threadIdx.x & (lanes - 1);
   const int groups = kNormThreads / lanes;
-  const int group = threadIdx.x / lanes;
   float w[kNv][kVec], b[kNv][kVec];
 #pragma unroll
   for (int j = 0; j < kNv; ++j) {
@@ -71,54 +129,39 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(const NormParams
     }
   }
   const float inv_c = 1.f / static_cast<float>(c);
-  const T* x = static_cast<const T*>(p.x);
   T* y = static_cast<T*>(p.y);
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * groups; r0 < p.n;
-       r0 += static_cast<int64_t>(gridDim.x) * groups) {
-    const int64_t r = r0 + group;
-    const bool row = r < p.n;
-    float v[kNv][kVec];
-    float sum = 0.f;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups * kU; base < p.n;
+       base += static_cast<int64_t>(gridDim.x) * groups * kU) {
+    const int64_t r0 = base + threadIdx.x / lanes;
+    NormRows<T, kVec, kNv, kU, kBlock> rows;
+    rows.load(static_cast<const T*>(p.x), p.x_stride, r0, p.n, groups, t, lanes, c);
+    float mean[kU], rstd[kU];
+    rows.stats(mean, rstd, t, lanes, c, inv_c, p.eps, red);
 #pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-      const int col = (t + lanes * j) * kVec;
-      load_vec<T, kVec>(x + r * p.x_stride + col, row && col < c, v[j]);
+    for (int k = 0; k < kU; ++k) {
+      const int64_t r = r0 + static_cast<int64_t>(k) * groups;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) sum += v[j][i];
-    }
-    const float mean = group_sum<kBlock>(sum, lanes, red) * inv_c;
-    float sq = 0.f;
+      for (int j = 0; j < kNv; ++j) {
+        const int col = (t + lanes * j) * kVec;
+        if (r < p.n && col < c) {
+          float o[kVec];
 #pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-      const bool in = (t + lanes * j) * kVec < c;
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        v[j][i] -= mean;
-        sq += in ? v[j][i] * v[j][i] : 0.f;
-      }
-    }
-    const float rstd = rsqrtf(group_sum<kBlock>(sq, lanes, red) * inv_c + p.eps);
-#pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-      const int col = (t + lanes * j) * kVec;
-      if (row && col < c) {
-        float o[kVec];
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) o[i] = v[j][i] * rstd * w[j][i] + b[j][i];
-        store_vec<T, kVec>(y + r * c + col, o);
+          for (int i = 0; i < kVec; ++i)
+            o[i] = (rows.x[k][j].get(i) - mean[k]) * rstd[k] * w[j][i] + b[j][i];
+          store_vec<T, kVec>(y + r * c + col, o);
+        }
       }
     }
   }
 }
 
-template <class T, int kVec, int kNv, bool kBlock>
+template <class T, int kVec, int kNv, int kU, bool kBlock>
 __global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(const NormParams p) {
   extern __shared__ float acc[];  // [2, C]: the block's parameter gradients
-  __shared__ float red[kNormThreads / 32];
+  __shared__ float red[kNormThreads / 32][kU];
   const int lanes = p.lanes, c = p.c;
   const int t = threadIdx.x & (lanes - 1);
   const int groups = kNormThreads / lanes;
-  const int group = threadIdx.x / lanes;
   float w[kNv][kVec], dw[kNv][kVec], db[kNv][kVec];
 #pragma unroll
   for (int j = 0; j < kNv; ++j) {
@@ -130,71 +173,72 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(const NormParams
     }
   }
   const float inv_c = 1.f / static_cast<float>(c);
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
   T* dx = static_cast<T*>(p.y);
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * groups; r0 < p.n;
-       r0 += static_cast<int64_t>(gridDim.x) * groups) {
-    const int64_t r = r0 + group;
-    const bool row = r < p.n;
-    float v[kNv][kVec], g[kNv][kVec];
-    float sum = 0.f;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups * kU; base < p.n;
+       base += static_cast<int64_t>(gridDim.x) * groups * kU) {
+    const int64_t r0 = base + threadIdx.x / lanes;
+    NormRows<T, kVec, kNv, kU, kBlock> rows, grads;
+    rows.load(static_cast<const T*>(p.x), p.x_stride, r0, p.n, groups, t, lanes, c);
+    grads.load(static_cast<const T*>(p.dy), p.dy_stride, r0, p.n, groups, t, lanes, c);
+    float mean[kU], rstd[kU], s1[kU], s2[kU];
+    rows.stats(mean, rstd, t, lanes, c, inv_c, p.eps, red);
 #pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-      const int col = (t + lanes * j) * kVec;
-      load_vec<T, kVec>(x + r * p.x_stride + col, row && col < c, v[j]);
-      load_vec<T, kVec>(dy + r * p.dy_stride + col, row && col < c, g[j]);
-    }
+    for (int k = 0; k < kU; ++k) {
+      s1[k] = s2[k] = 0.f;
+      if (r0 + static_cast<int64_t>(k) * groups < p.n) {  // rows past the end add nothing
 #pragma unroll
-    for (int j = 0; j < kNv; ++j)
+        for (int j = 0; j < kNv; ++j) {
+          if ((t + lanes * j) * kVec < c) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) sum += v[j][i];
-    const float mean = group_sum<kBlock>(sum, lanes, red) * inv_c;
-    float sq = 0.f;
-#pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-      const bool in = (t + lanes * j) * kVec < c;
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        v[j][i] = in ? v[j][i] - mean : 0.f;
-        sq += v[j][i] * v[j][i];
-      }
-    }
-    const float rstd = rsqrtf(group_sum<kBlock>(sq, lanes, red) * inv_c + p.eps);
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        v[j][i] *= rstd;
-        if (row) {  // rows past the end add nothing
-          db[j][i] += g[j][i];
-          dw[j][i] += g[j][i] * v[j][i];
+            for (int i = 0; i < kVec; ++i) {
+              const float z = (rows.x[k][j].get(i) - mean[k]) * rstd[k], g = grads.x[k][j].get(i);
+              db[j][i] += g;
+              dw[j][i] += g * z;
+              s1[k] += g * w[j][i];
+              s2[k] += g * w[j][i] * z;
+            }
+          }
         }
-        g[j][i] *= w[j][i];
-        s1 += g[j][i];
-        s2 += g[j][i] * v[j][i];
       }
     }
-    s1 = group_sum<kBlock>(s1, lanes, red) * inv_c;
-    s2 = group_sum<kBlock>(s2, lanes, red) * inv_c;
+    group_sum<kBlock>(s1, lanes, red);
+    group_sum<kBlock>(s2, lanes, red);
 #pragma unroll
-    for (int j = 0; j < kNv; ++j) {
-      const int col = (t + lanes * j) * kVec;
-      if (row && col < c && dx) {
-        float o[kVec];
+    for (int k = 0; k < kU; ++k) {
+      const int64_t r = r0 + static_cast<int64_t>(k) * groups;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) o[i] = rstd * (g[j][i] - s1 - v[j][i] * s2);
-        store_vec<T, kVec>(dx + r * c + col, o);
+      for (int j = 0; j < kNv; ++j) {
+        const int col = (t + lanes * j) * kVec;
+        if (r < p.n && col < c && dx) {
+          float o[kVec];
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            const float z = (rows.x[k][j].get(i) - mean[k]) * rstd[k];
+            o[i] = rstd[k] * (grads.x[k][j].get(i) * w[j][i] - s1[k] * inv_c - z * (s2[k] * inv_c));
+          }
+          store_vec<T, kVec>(dx + r * c + col, o);
+        }
       }
     }
   }
   if (p.partial == nullptr) return;
   // The block's groups add their sums one after another, so the order of the
-  // additions is fixed.
-  for (int turn = 0; turn < groups; ++turn) {
+  // additions is fixed; within a warp, by exchanges.
+  const int per_warp = lanes < 32 ? 32 / lanes : 1;
+#pragma unroll
+  for (int j = 0; j < kNv; ++j) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      for (int off = lanes; off < 32; off <<= 1) {
+        dw[j][i] += __shfl_xor_sync(0xffffffffu, dw[j][i], off);
+        db[j][i] += __shfl_xor_sync(0xffffffffu, db[j][i], off);
+      }
+    }
+  }
+  const int turns = groups / per_warp, mine = threadIdx.x / lanes;
+  for (int turn = 0; turn < turns; ++turn) {
     __syncthreads();
-    if (group == turn) {
+    if (mine == turn * per_warp) {
 #pragma unroll
       for (int j = 0; j < kNv; ++j) {
 #pragma unroll
@@ -247,12 +291,6 @@ int check_norm(const TgsLayerNormArgs* a, const char* who) {
   return TGS_OK;
 }
 
-int norm_blocks(int64_t n, int lanes) {
-  const int64_t groups = kNormThreads / lanes;
-  return static_cast<int>(std::min<int64_t>(ceil_div<int64_t>(n, groups),
-                                            static_cast<int64_t>(sm_count()) * 8));
-}
-
 // Threads per row: the fewest neighbours (a power of two) that hold it with
 // kNv loads each.
 int norm_lanes(int c, int per_thread) {
@@ -261,32 +299,50 @@ int norm_lanes(int c, int per_thread) {
   return lanes;
 }
 
-template <class T, int kVec, int kNv, bool kBlock, bool kBwd>
+template <class T, int kVec, int kNv, int kU, bool kBlock, bool kBwd>
 int launch_norm(NormParams p, cudaStream_t s, int* blocks) {
   p.lanes = kBlock ? kNormThreads : norm_lanes(p.c, kVec * kNv);
-  *blocks = norm_blocks(p.n, p.lanes);
+  const int64_t rows = static_cast<int64_t>(kNormThreads / p.lanes) * kU;
+  // Blocks that are resident at once; the backward's also bound the partial
+  // sums. Register use leaves two to eight to an SM.
+  const int64_t most = static_cast<int64_t>(sm_count()) * kNormBlocksPerSm;
+  *blocks = static_cast<int>(std::min<int64_t>(ceil_div<int64_t>(p.n, rows), most));
   if constexpr (kBwd) {
     const int smem = p.partial ? 2 * p.c * static_cast<int>(sizeof(float)) : 0;
-    TGS_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<T, kVec, kNv, kBlock>,
-                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    norm_bwd_kernel<T, kVec, kNv, kBlock><<<*blocks, kNormThreads, smem, s>>>(p);
+    if (smem > 48 * 1024)
+      TGS_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<T, kVec, kNv, kU, kBlock>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    norm_bwd_kernel<T, kVec, kNv, kU, kBlock><<<*blocks, kNormThreads, smem, s>>>(p);
   } else {
-    norm_fwd_kernel<T, kVec, kNv, kBlock><<<*blocks, kNormThreads, 0, s>>>(p);
+    norm_fwd_kernel<T, kVec, kNv, kU, kBlock><<<*blocks, kNormThreads, 0, s>>>(p);
   }
   TGS_LAUNCH_CHECK();
   return TGS_OK;
 }
 
+// kNv and kU: a thread keeps about 64 bytes of each of its tensors on their
+// way, and no more values than its registers hold (the backward has four sets).
 template <class T, int kVec, bool kBwd>
 int launch_norm_vec(const NormParams& p, cudaStream_t s, int* blocks) {
-  constexpr int kWarp = 32 * kVec;  // values that one load of a warp covers
-  if (p.c <= kWarp) return launch_norm<T, kVec, 1, false, kBwd>(p, s, blocks);
-  if (p.c <= 2 * kWarp) return launch_norm<T, kVec, 2, false, kBwd>(p, s, blocks);
-  if (p.c <= 4 * kWarp) return launch_norm<T, kVec, 4, false, kBwd>(p, s, blocks);
-  constexpr int kWide = kNormMaxC / (kNormThreads * kVec);
-  if (p.c <= kNormThreads * kVec * (kWide / 4 > 0 ? kWide / 4 : 1))
-    return launch_norm<T, kVec, (kWide / 4 > 0 ? kWide / 4 : 1), true, kBwd>(p, s, blocks);
-  return launch_norm<T, kVec, kWide, true, kBwd>(p, s, blocks);
+  constexpr int kWarp = 32 * kVec, kWide = kNormThreads * kVec;  // values of one load
+  constexpr bool kOne = kVec == 1;
+  const int c = p.c;
+  if (c <= kWarp) return launch_norm<T, kVec, 1, kBwd ? 2 : 4, false, kBwd>(p, s, blocks);
+  if (c <= 2 * kWarp) return launch_norm<T, kVec, 2, kOne ? 4 : kBwd ? 1 : 2, false, kBwd>(p, s, blocks);
+  if constexpr (sizeof(T) * kVec == 16 && sizeof(T) == 2) {
+    if (c <= 3 * kWarp) return launch_norm<T, kVec, 3, 1, false, kBwd>(p, s, blocks);
+  }
+  if (c <= 4 * kWarp) return launch_norm<T, kVec, 4, kOne && !kBwd ? 2 : 1, false, kBwd>(p, s, blocks);
+  if constexpr (kOne) {
+    if (c <= 8 * kWarp) return launch_norm<T, kVec, 8, 1, false, kBwd>(p, s, blocks);
+    if (c <= 2 * kWide) return launch_norm<T, kVec, 2, 4, true, kBwd>(p, s, blocks);
+    if (c <= 4 * kWide) return launch_norm<T, kVec, 4, 2, true, kBwd>(p, s, blocks);
+    return launch_norm<T, kVec, 32, 1, true, kBwd>(p, s, blocks);
+  } else {
+    if (c <= kWide) return launch_norm<T, kVec, 1, 4, true, kBwd>(p, s, blocks);
+    if (c <= 2 * kWide) return launch_norm<T, kVec, 2, 2, true, kBwd>(p, s, blocks);
+    return launch_norm<T, kVec, kNormMaxC / kWide, 1, true, kBwd>(p, s, blocks);
+  }
 }
 
 template <class T, bool kBwd>
@@ -329,7 +385,7 @@ extern "C" int tgs_layer_norm_fwd(const TgsLayerNormArgs* a, void* stream) {
 
 extern "C" int64_t tgs_layer_norm_scratch_floats(int64_t n, int32_t c) {
   if (n <= 0 || c <= 0) return 0;
-  return std::min<int64_t>(n, static_cast<int64_t>(sm_count()) * 8) * 2 * c;
+  return std::min<int64_t>(n, static_cast<int64_t>(sm_count()) * kNormBlocksPerSm) * 2 * c;
 }
 
 extern "C" int tgs_layer_norm_bwd(const TgsLayerNormBwdArgs* b, void* stream) {

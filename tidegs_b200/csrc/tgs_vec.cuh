@@ -44,6 +44,26 @@ __device__ __forceinline__ void load_vec(const T* p, bool on, float (&v)[kVec]) 
   }
 }
 
+// kVec values as they lie in memory.
+template <class T, int kVec>
+struct Packed {
+  static constexpr bool kWhole = sizeof(T) * kVec == 16;
+  union {
+    uint4 q;
+    T t[kVec];
+  };
+  __device__ __forceinline__ Packed() {}
+  __device__ __forceinline__ void load(const T* p, bool on) {
+    if constexpr (kWhole) {
+      q = on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) t[i] = on ? p[i] : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const { return to_f32(t[i]); }
+};
+
 template <class T, int kVec>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[kVec]) {
   if constexpr (sizeof(T) * kVec == 16) {
