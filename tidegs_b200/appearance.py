@@ -45,7 +45,8 @@ def _check(t: torch.Tensor, who: str, name: str, device: Optional[torch.device] 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """t as [n, width] rows of contiguous values (a copy where it has none)."""
-    t = t.detach()
+    if t.is_contiguous():
+        return t if t.dim() == 2 else t.view(-1, width)
     t = t if t.dim() == 2 else t.reshape(-1, width)
     if t.stride(1) == 1 or width == 1:
         if t.shape[0] <= 1 or t.stride(0) >= width:
@@ -54,18 +55,20 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+    n, width = t.shape
+    return t.stride(0) if n > 1 else width
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
     """The device as the current one (no call where it is already)."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
@@ -78,7 +81,8 @@ def _norm_args(x, weight, bias, eps) -> "_lib.LayerNormArgs":
     param = weight if weight is not None else bias
     a = _lib.LayerNormArgs()
     a.x, a.weight, a.bias = x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias)
-    a.n, a.c, a.x_stride = int(x.shape[0]), int(x.shape[1]), _row_stride(x)
+    a.n, a.c = x.shape
+    a.x_stride = _row_stride(x)
     a.dtype = _lib.DTYPES[x.dtype]
     a.param_dtype = _lib.DTYPES[param.dtype if param is not None else x.dtype]
     a.eps = eps
@@ -87,8 +91,8 @@ def _norm_args(x, weight, bias, eps) -> "_lib.LayerNormArgs":
 
 def _norm_forward(x, weight, bias, eps):
     rows = _rows(x, x.shape[-1])
-    weight = None if weight is None else weight.detach().contiguous()
-    bias = None if bias is None else bias.detach().contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     a = _norm_args(rows, weight, bias, eps)
     a.y = y.data_ptr()
@@ -112,7 +116,7 @@ class _LayerNorm(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         c = x.shape[-1]
         rows, v_rows = _rows(x, c), _rows(v_y, c)
-        weight = None if weight is None else weight.detach().contiguous()
+        weight = None if weight is None else weight.contiguous()
         ptype = weight.dtype if weight is not None else ctx.bias if ctx.bias else x.dtype
         v_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
         v_w = torch.empty(c, dtype=ptype, device=x.device) if need_w else None
@@ -207,7 +211,7 @@ def _ffn_args(x, w_gate, w_up, w_down, backward: bool):
 
 def _ffn_forward(x, w_gate, w_up, w_down):
     rows = _rows(x, x.shape[-1])
-    weights = [w.detach().contiguous() for w in (w_gate, w_up, w_down)]
+    weights = [w.contiguous() for w in (w_gate, w_up, w_down)]
     y = torch.empty((*x.shape[:-1], w_down.shape[0]), dtype=x.dtype, device=x.device)
     with _on(x.device):
         a, _scratch = _ffn_args(rows, *weights, backward=False)
@@ -226,7 +230,7 @@ class _GatedFeedForward(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, v_y):
         x, *weights = ctx.saved_tensors
-        weights = [w.detach().contiguous() for w in weights]
+        weights = [w.contiguous() for w in weights]
         need_x, *need_w = ctx.needs_input_grad
         d, o = x.shape[-1], weights[2].shape[0]
         rows, v_rows = _rows(x, d), _rows(v_y, o)
@@ -280,7 +284,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 def _dropout_run(x, p, seed, offset, ids, per_row):
     n = int(x.shape[0])
     c = x.numel() // n if n else 1
-    rows = _rows(x.detach().reshape(n, c) if x.dim() != 2 else x, c)
+    rows = _rows(x.reshape(n, c) if x.dim() != 2 else x, c)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     a = _lib.DropoutArgs()
     a.x, a.y, a.ids = rows.data_ptr(), y.data_ptr(), _lib.ptr(ids)

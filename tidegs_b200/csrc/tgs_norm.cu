@@ -257,26 +257,31 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(const NormParams
     p.partial[static_cast<int64_t>(blockIdx.x) * 2 * c + e] = acc[e];
 }
 
-// Column sums of the blocks' partial gradients: 32 columns per block, eight
+// Column sums of the blocks' partial gradients: 32 columns per block, 32
 // threads per column.
-__global__ void __launch_bounds__(256) norm_param_kernel(const float* __restrict__ partial,
-                                                         int blocks, int c, int dtype,
-                                                         void* dweight, void* dbias) {
-  __shared__ float s[8][33];
-  const int e = blockIdx.x * 32 + (threadIdx.x & 31);
-  const int k = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) norm_param_kernel(const float* __restrict__ partial,
+                                                          int blocks, int c, int dtype,
+                                                          void* dweight, void* dbias) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int e = blockIdx.x * 32 + lane;
   float sum = 0.f;
-  if (e < 2 * c)
-    for (int b = k; b < blocks; b += 8) sum += partial[static_cast<int64_t>(b) * 2 * c + e];
-  s[k][threadIdx.x & 31] = sum;
+  if (e < 2 * c) {
+#pragma unroll 4
+    for (int b = k; b < blocks; b += 32) sum += partial[static_cast<int64_t>(b) * 2 * c + e];
+  }
+  s[k][lane] = sum;
   __syncthreads();
-  if (k != 0 || e >= 2 * c) return;
+  // column k of the block's 32: its 32 partial sums, added as a tree
+  sum = s[lane][k];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) sum += s[i][threadIdx.x & 31];
-  if (e < c) {
-    if (dweight) store_param(dweight, dtype, e, sum);
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  const int col = blockIdx.x * 32 + k;
+  if (lane != 0 || col >= 2 * c) return;
+  if (col < c) {
+    if (dweight) store_param(dweight, dtype, col, sum);
   } else if (dbias) {
-    store_param(dbias, dtype, e - c, sum);
+    store_param(dbias, dtype, col - c, sum);
   }
 }
 
@@ -301,44 +306,49 @@ int norm_lanes(int c, int per_thread) {
 
 template <class T, int kVec, int kNv, int kU, bool kBlock, bool kBwd>
 int launch_norm(NormParams p, cudaStream_t s, int* blocks) {
+  const auto kernel = kBwd ? norm_bwd_kernel<T, kVec, kNv, kU, kBlock>
+                           : norm_fwd_kernel<T, kVec, kNv, kU, kBlock>;
   p.lanes = kBlock ? kNormThreads : norm_lanes(p.c, kVec * kNv);
   const int64_t rows = static_cast<int64_t>(kNormThreads / p.lanes) * kU;
-  // Blocks that are resident at once; the backward's also bound the partial
-  // sums. Register use leaves two to eight to an SM.
-  const int64_t most = static_cast<int64_t>(sm_count()) * kNormBlocksPerSm;
-  *blocks = static_cast<int>(std::min<int64_t>(ceil_div<int64_t>(p.n, rows), most));
-  if constexpr (kBwd) {
-    const int smem = p.partial ? 2 * p.c * static_cast<int>(sizeof(float)) : 0;
-    if (smem > 48 * 1024)
-      TGS_CUDA(cudaFuncSetAttribute(norm_bwd_kernel<T, kVec, kNv, kU, kBlock>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    norm_bwd_kernel<T, kVec, kNv, kU, kBlock><<<*blocks, kNormThreads, smem, s>>>(p);
-  } else {
-    norm_fwd_kernel<T, kVec, kNv, kU, kBlock><<<*blocks, kNormThreads, 0, s>>>(p);
+  const int smem = kBwd && p.partial ? 2 * p.c * static_cast<int>(sizeof(float)) : 0;
+  if (smem > 48 * 1024)
+    TGS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // As many blocks as are resident at once: each sums its parameter gradients
+  // and hands them over once.
+  static int resident = 0;
+  if (resident == 0) {
+    int n = 0;
+    TGS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kNormThreads, 0));
+    resident = std::max(1, std::min(n, kNormBlocksPerSm));
   }
+  *blocks = static_cast<int>(std::min<int64_t>(ceil_div<int64_t>(p.n, rows),
+                                               static_cast<int64_t>(sm_count()) * resident));
+  kernel<<<*blocks, kNormThreads, smem, s>>>(p);
   TGS_LAUNCH_CHECK();
   return TGS_OK;
 }
 
-// kNv and kU: a thread keeps about 64 bytes of each of its tensors on their
-// way, and no more values than its registers hold (the backward has four sets).
+// kNv and kU: few threads to a row, for few exchanges (at 59 columns of fp32,
+// 8 threads of 8 values against 32 of 2), while a thread keeps about 64 bytes
+// of each of its tensors on their way and no more values than its registers
+// hold (the backward has four sets).
 template <class T, int kVec, bool kBwd>
 int launch_norm_vec(const NormParams& p, cudaStream_t s, int* blocks) {
   constexpr int kWarp = 32 * kVec, kWide = kNormThreads * kVec;  // values of one load
-  constexpr bool kOne = kVec == 1;
   const int c = p.c;
-  if (c <= kWarp) return launch_norm<T, kVec, 1, kBwd ? 2 : 4, false, kBwd>(p, s, blocks);
-  if (c <= 2 * kWarp) return launch_norm<T, kVec, 2, kOne ? 4 : kBwd ? 1 : 2, false, kBwd>(p, s, blocks);
-  if constexpr (sizeof(T) * kVec == 16 && sizeof(T) == 2) {
-    if (c <= 3 * kWarp) return launch_norm<T, kVec, 3, 1, false, kBwd>(p, s, blocks);
-  }
-  if (c <= 4 * kWarp) return launch_norm<T, kVec, 4, kOne && !kBwd ? 2 : 1, false, kBwd>(p, s, blocks);
-  if constexpr (kOne) {
-    if (c <= 8 * kWarp) return launch_norm<T, kVec, 8, 1, false, kBwd>(p, s, blocks);
-    if (c <= 2 * kWide) return launch_norm<T, kVec, 2, 4, true, kBwd>(p, s, blocks);
+  if constexpr (kVec == 1) {
+    if (c <= 4) return launch_norm<T, kVec, 4, kBwd ? 2 : 4, false, kBwd>(p, s, blocks);
+    if (c <= 8 * kWarp) return launch_norm<T, kVec, 8, kBwd ? 1 : 2, false, kBwd>(p, s, blocks);
+    if (c <= 16 * kWarp) return launch_norm<T, kVec, 16, 1, false, kBwd>(p, s, blocks);
     if (c <= 4 * kWide) return launch_norm<T, kVec, 4, 2, true, kBwd>(p, s, blocks);
     return launch_norm<T, kVec, 32, 1, true, kBwd>(p, s, blocks);
   } else {
+    if (c <= 4 * kVec) return launch_norm<T, kVec, 1, kBwd ? 2 : 4, false, kBwd>(p, s, blocks);
+    if (c <= 2 * kWarp) return launch_norm<T, kVec, 2, kBwd ? 1 : 2, false, kBwd>(p, s, blocks);
+    if constexpr (sizeof(T) == 2) {
+      if (c <= 3 * kWarp) return launch_norm<T, kVec, 3, 1, false, kBwd>(p, s, blocks);
+    }
+    if (c <= 4 * kWarp) return launch_norm<T, kVec, 4, 1, false, kBwd>(p, s, blocks);
     if (c <= kWide) return launch_norm<T, kVec, 1, 4, true, kBwd>(p, s, blocks);
     if (c <= 2 * kWide) return launch_norm<T, kVec, 2, 2, true, kBwd>(p, s, blocks);
     return launch_norm<T, kVec, kNormMaxC / kWide, 1, true, kBwd>(p, s, blocks);
@@ -405,7 +415,7 @@ extern "C" int tgs_layer_norm_bwd(const TgsLayerNormBwdArgs* b, void* stream) {
     if (int rc = launch_norm_any<true>(p, a.dtype, s, &blocks)) return rc;
   }
   if (params) {
-    norm_param_kernel<<<ceil_div(2 * a.c, 32), 256, 0, s>>>(b->scratch, blocks, a.c, a.param_dtype,
+    norm_param_kernel<<<ceil_div(2 * a.c, 32), 1024, 0, s>>>(b->scratch, blocks, a.c, a.param_dtype,
                                                            b->v_weight, b->v_bias);
     TGS_LAUNCH_CHECK();
   }
