@@ -166,33 +166,6 @@ __device__ __forceinline__ float fast_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// Two fp32 values in a register pair: one instruction for both.
-struct F2 {
-  uint64_t v;
-  __device__ __forceinline__ F2(float a, float b) {
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  }
-  __device__ __forceinline__ explicit F2(uint64_t x) : v(x) {}
-  __device__ __forceinline__ void get(float& a, float& b) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  }
-};
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
-  return F2(r);
-}
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
-  return F2(r);
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return F2(r);
-}
-
 // 1 / (1 + exp(-g)) of two values. The special-function unit (16 results a
 // cycle and SM) bounds the activation, so they share a reciprocal, 1 / a =
 // b / (a b): 1.5 of its operations a value instead of 2. Where the product
