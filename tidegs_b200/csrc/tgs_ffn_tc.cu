@@ -227,21 +227,24 @@ __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint
 }
 
 // A row tile -> operand blocks, by threads: for matrices that no tensor map
-// can describe. Thread -> one 16-byte unit of every 16th row of a block.
+// can describe. As many neighbouring threads to a row as it has 16-byte units
+// in the block (a power of two), so that narrow rows go many at a time.
 __device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src, int64_t stride,
                                           int64_t r0, int64_t n, int cols, int k16, int tid) {
-  static_assert(kLoad == 128, "sixteen rows of eight units per pass");
-  const int unit = tid & 7;
-  for (int c = 0; 8 * c < 2 * k16; ++c) {
-    if (unit >= 2 * k16 - 8 * c) continue;
+  for (int c = 0; 4 * c < k16; ++c) {
+    const int left_units = 2 * k16 - 8 * c;
+    const int per_row = left_units > 4 ? 8 : left_units > 2 ? 4 : 2;
+    const int unit = tid & (per_row - 1), rows = kLoad / per_row;
+    if (unit >= left_units) continue;
     const int col = c * kBlockCols + unit * 8;
-    uint32_t at = dst + c * kBlockBytes + unit_offset(tid >> 3, unit);
-    const __nv_bfloat16* from = src + (r0 + (tid >> 3)) * stride + col;
-    int64_t left = n - r0 - (tid >> 3);
-#pragma unroll 2
-    for (int i = 0; i < kTile / 16; ++i) {
-      st_shared16(at, left > 0 ? load_unit(from, 0, cols - col, false) : make_uint4(0, 0, 0, 0));
-      at += 2048, from += 16 * stride, left -= 16;
+    int row = tid / per_row;
+    const __nv_bfloat16* from = src + (r0 + row) * stride + col;
+    int64_t left = n - r0 - row;
+#pragma unroll 4
+    for (int i = 0; i < per_row; ++i) {
+      st_shared16(dst + c * kBlockBytes + unit_offset(row, unit),
+                  left > 0 ? load_unit(from, 0, cols - col, false) : make_uint4(0, 0, 0, 0));
+      row += rows, from += rows * stride, left -= rows;
     }
   }
 }
