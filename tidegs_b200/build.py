@@ -26,7 +26,8 @@ LIB_PATH = LIB_DIR / "libtidegs_b200.so"
 
 SOURCES = ("tgs_abi.cu", "tgs_adam.cu", "tgs_blocks.cu", "tgs_dirty.cu", "tgs_exchange.cu",
            "tgs_sparse.cu", "tgs_cull.cu", "tgs_render.cu", "tgs_sh.cu", "tgs_norm.cu",
-           "tgs_ffn.cu", "tgs_ffn_tc.cu", "tgs_dropout.cu")
+           "tgs_ffn.cu", "tgs_ffn_tc.cu", "tgs_ffn_tc32.cu",
+           "tgs_dropout.cu")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3",

@@ -429,7 +429,24 @@ int launch_weights(const FfnParams& p, int slices, cudaStream_t s) {
   return TGS_OK;
 }
 
+// Whether a 32-bit call takes the tensor cores.
+bool large_f32(int64_t n, int d, int h, int o) {
+  (void)d, (void)h, (void)o;
+  return n >= 4096;
+}
+
+int sum_slices(const FfnParams& p, int slices, cudaStream_t s) {
+  const int64_t all = static_cast<int64_t>(p.h) * (2 * p.d + p.o);
+  ffn_weights_sum_kernel<<<static_cast<unsigned>(ceil_div<int64_t>(all, 32)), kThreads, 0, s>>>(p, slices);
+  TGS_LAUNCH_CHECK();
+  return TGS_OK;
+}
+
 int ffn_backward_f32(const FfnParams& p, cudaStream_t s) {
+  if (large_f32(p.n, p.d, p.h, p.o)) {
+    if (int rc = ffn_tc32_run(p, true, s)) return rc;
+    return p.dwg ? sum_slices(p, tc32_slices(p.n, p.d, p.h, p.o), s) : TGS_OK;
+  }
   if (p.y) {
     if (int rc = rows_f32<true>(p, s)) return rc;
   }
@@ -441,11 +458,7 @@ int ffn_backward_f32(const FfnParams& p, cudaStream_t s) {
     case 4: rc = launch_weights<4, 8>(p, slices, s); break;
     default: rc = launch_weights<2, 16>(p, slices, s); break;
   }
-  if (rc) return rc;
-  const int64_t all = static_cast<int64_t>(p.h) * (2 * p.d + p.o);
-  ffn_weights_sum_kernel<<<static_cast<unsigned>(ceil_div<int64_t>(all, 32)), kThreads, 0, s>>>(p, slices);
-  TGS_LAUNCH_CHECK();
-  return TGS_OK;
+  return rc ? rc : sum_slices(p, slices, s);
 }
 
 int check_ffn(const TgsFfnArgs* a, const char* who) {
@@ -479,8 +492,11 @@ extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32
                                           int32_t backward) {
   if (n <= 0 || d <= 0 || h <= 0 || o <= 0) return 0;
   if (dtype != TGS_F32) return ffn_tc_scratch_floats(n, d, h, o, backward != 0);
-  if (!backward) return 0;
-  return weights_floats(n, d, h, o);
+  const bool large = large_f32(n, d, h, o);
+  if (!backward) return large ? tc32_hidden_floats(n, h, false) : 0;
+  if (!large) return weights_floats(n, d, h, o);
+  return ceil_div<int64_t>(tc32_slices(n, d, h, o) * static_cast<int64_t>(h) * (2 * d + o), 4) * 4 +
+         tc32_hidden_floats(n, h, true);
 }
 
 extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
@@ -492,7 +508,7 @@ extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
   const FfnParams p = ffn_params(*a);
   cudaStream_t s = as_stream(stream);
   if (a->dtype == TGS_BF16) return ffn_tc_forward(p, s);
-  return rows_f32<false>(p, s);
+  return large_f32(p.n, p.d, p.h, p.o) ? ffn_tc32_run(p, false, s) : rows_f32<false>(p, s);
 }
 
 extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {

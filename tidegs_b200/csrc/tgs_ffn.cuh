@@ -21,4 +21,11 @@ int ffn_tc_forward(const FfnParams& p, cudaStream_t s);
 int64_t ffn_tc_scratch_floats(int64_t n, int d, int h, int o, bool backward);
 int ffn_tc_backward(const FfnParams& p, cudaStream_t s);
 
+// fp32 on the tensor cores (tgs_ffn_tc32.cu): Y or dX, and partial weights'
+// gradients in `tc32_slices` slices [dWg [H, D] | dWu [H, D] | dWd^T [H, O]] at
+// the start of the scratch.
+int ffn_tc32_run(const FfnParams& p, bool backward, cudaStream_t s);
+int tc32_slices(int64_t n, int d, int h, int o);
+int64_t tc32_hidden_floats(int64_t n, int h, bool backward);
+
 }  // namespace tgs
