@@ -9,24 +9,25 @@
 // go through memory, in batches of rows small enough to stay in L2: one launch
 // makes the hidden values, one the output, one the weights' gradients.
 //
-// A block makes one 128 x 128 tile of a product. Eight warps load and split
-// (the next stage's values are in registers while the tensor cores work on
-// this one) and later store the result; one issues the matrix instructions.
-// Bound: the matrix instructions where the contracted width is long (measured
-// rates stand at the plan below).
+// A block makes one 128 x 128 tile of a product. Sixteen warps load and split,
+// and store the result; one issues the matrix instructions. The accumulators
+// round towards zero: 96 additions to one left 2.4e-6 of the result, 192
+// 5.7e-6. So a stage's products, the smallest first, get accumulators of their
+// own (two take turns) and are added in registers, where additions round to
+// the nearest.
 #include "tgs_ffn.cuh"
 #include "tgs_tc.cuh"
 
 namespace tgs {
 namespace {
 
-constexpr int kWorkers = 256;
+constexpr int kWorkers = 512;
 constexpr int kThreads32 = kWorkers + 32;
 constexpr int kTile = 128;
 constexpr int kStep = 64;             // contracted values per stage
 constexpr int kPart = kBlockBytes;    // one operand's part of a stage
 constexpr int kStage = 6 * kPart;     // A's three parts, then B's
-constexpr int kSums = 16;             // stages between two additions in 32 bits
+constexpr int kUnits = 1024 / kWorkers;  // of eight values, per operand, thread and stage
 
 enum : int { kHidden = 0, kHiddenBwd = 1, kOutput = 2, kWeights = 3 };
 
@@ -100,11 +101,11 @@ __device__ __forceinline__ bool vec_rows(const Mat& m) { return aligned16(m.p) &
 template <int kJob>
 __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_constant__ Tc32Params p) {
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[2], empty[2], sums, drained;
+  __shared__ uint64_t full[2], done[2], drained[2];
   __shared__ uint32_t tmem_slot;
   constexpr bool kMn = kJob == kWeights;           // both operands by rows
   constexpr bool kHid = kJob <= kHiddenBwd;
-  constexpr uint32_t kCols = kJob == kHiddenBwd ? 256 : 128;
+  constexpr uint32_t kCols = 256;  // two accumulators
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -139,8 +140,10 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
   if (warp == kWorkers / 32) {
     tmem_alloc(&tmem_slot, kCols);
     if (lane == 0) {
-      for (int i = 0; i < 2; ++i) mbar_init(&full[i], kWorkers / 32), mbar_init(&empty[i], 1);
-      mbar_init(&sums, 1), mbar_init(&drained, kWorkers / 32);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&full[i], kWorkers / 32), mbar_init(&done[i], 1);
+        mbar_init(&drained[i], kWorkers / 32);
+      }
       fence_mbar_init();
     }
   }
@@ -158,23 +161,48 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
 
   if (warp < kWorkers / 32) {
     const int tid = threadIdx.x;
-    // kSums stages are summed by the tensor cores, then added to these.
-    float sum[64];
-    if constexpr (kMn) {
-#pragma unroll
-      for (int i = 0; i < 64; ++i) sum[i] = 0.f;
-    }
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-    int term = which, k0 = 0, drains = 0;
-    Unit a[4], b[4];
+    const int row = (warp & 3) * 32 + lane, part = warp >> 2;  // a quarter of the columns
+    // hidden: 16 columns of G, U and dH; else 32 of the tile
+    float sum[3][16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[0][i] = sum[1][i] = sum[2][i] = 0.f;
+    auto add = [&](int col, float (&to)[16]) {
+      float v[16];
+      tmem_ld(acc + quarter + col, v);
+      tmem_wait_ld(v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) to[i] += v[i];
+    };
+    // Adds stage s, which belongs to term `of`.
+    auto drain = [&](int s, int of) {
+      wait(&done[s & 1], s >> 1);
+      tc_fence_after();
+      const int at = (s & 1) * 128;
+      if constexpr (kHid) {
+        if (kJob == kHiddenBwd && of == 1) {
+          add(at + 16 * part, sum[2]);
+        } else {
+          add(at + 16 * part, sum[0]);
+          add(at + 64 + 16 * part, sum[1]);
+        }
+      } else {
+        if (32 * part < n) add(at + 32 * part, sum[0]);
+        if (32 * part + 16 < n) add(at + 32 * part + 16, sum[1]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&drained[s & 1]);
+    };
+    int term = which, k0 = 0;
+    Unit a[kUnits], b[kUnits];
     auto load = [&] {
       const Term& t = p.t[term];
       if constexpr (kMn) {  // [64 rows][128 columns] of each
         const int64_t r0 = k_begin + k0;
         const bool va = vec_rows(t.a), vb = vec_rows(t.b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kUnits; ++i) {
           const int e = tid + i * kWorkers, r = e >> 4, unit = e & 15;
           a[i] = load_values(t.a, r0 + r, k_end, static_cast<int>(m0) + unit * 8, va);
           b[i] = load_values(t.b, r0 + r, k_end, n0 + unit * 8, vb);
@@ -184,7 +212,7 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
         // B by rows: the second term of the hidden values, and dX's terms
         const bool b_mn = kJob == kHiddenBwd ? term == 1 : kJob == kOutput && p.d > 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kUnits; ++i) {
           const int e = tid + i * kWorkers;
           a[i] = load_values(t.a, m0 + (e >> 3), t.a.rows, k0 + (e & 7) * 8, va);
           if (b_mn) {
@@ -200,15 +228,14 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
       k0 += kStep;
       if (!kMn && k0 >= t.k) k0 = 0, ++term;
     };
-    int used = term;
+    int used = term, before = term;
     if (total > 0) load();
     for (int s = 0; s < total; ++s) {
-      const int st = s & 1;
-      if (s >= 2) wait(&empty[st], (s >> 1) - 1);
-      const uint32_t to = base + (p.stages == 2 ? st : 0) * kStage;
+      // the stage that last used this half of shared memory has been drained
+      const uint32_t to = base + (p.stages == 2 ? s & 1 : 0) * kStage;
       const bool b_mn = kMn || (kJob == kHiddenBwd ? used == 1 : kJob == kOutput && p.d > 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kUnits; ++i) {
         const int e = tid + i * kWorkers;
         const uint32_t k_at = unit_offset(e >> 3, e & 7);
         const uint32_t mn_at = ((e >> 3) & 1) * (kPart / 2) + unit_offset(e >> 4, e & 7);
@@ -217,146 +244,87 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st]);
+      if (lane == 0) mbar_arrive(&full[s & 1]);
+      const int of = used;
       used = term;
       if (s + 1 < total) load();
-      if constexpr (kMn) {
-        if ((s + 1) % kSums == 0 || s + 1 == total) {
-          wait(&sums, drains++);
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v[16];
-            if (half * 64 + 16 * c < n) {
-              tmem_ld(acc + quarter + half * 64 + 16 * c, v);
-              tmem_wait_ld(v);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) sum[16 * c + i] += v[i];
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&drained);
-        }
-      }
+      if (s > 0) drain(s - 1, before);
+      before = of;
     }
+    if (total > 0) drain(total - 1, before);
+    const int64_t r = m0 + row;
     if constexpr (kMn) {
-      const int hid = static_cast<int>(m0) + row;
-      if (hid < p.h) {
+      if (r < p.h) {
         const int64_t hd = static_cast<int64_t>(p.h) * p.d;
         const int width = which < 2 ? p.d : p.o;
         float* to = p.out[0] + blockIdx.x * (2 * hd + static_cast<int64_t>(p.h) * p.o) + which * hd +
-                    static_cast<int64_t>(hid) * width;
+                    r * width;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const int c = n0 + half * 64 + i;
-          if (c < width) to[c] = p.first ? sum[i] : to[c] + sum[i];
+        for (int i = 0; i < 32; ++i) {
+          const int c = n0 + 32 * part + i;
+          const float v = sum[i >> 4][i & 15];
+          if (c < width) to[c] = p.first ? v : to[c] + v;
+        }
+      }
+    } else if constexpr (kHid) {
+      const int c = n0 + 16 * part;
+      if (r < p.rows && c < p.h) {
+        float* to = p.out[0] + r * p.out_ld + c;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          float h[4], dg[4], du[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = sum[0][i + k], u = sum[1][i + k], d = sum[2][i + k];
+            const float sg = __fdividef(1.f, 1.f + __expf(-x)), act = x * sg;
+            h[k] = act * u;
+            dg[k] = d * u * (sg + act * (1.f - sg));
+            du[k] = d * act;
+          }
+          *reinterpret_cast<float4*>(to + i) = make_float4(h[0], h[1], h[2], h[3]);
+          if constexpr (kJob == kHiddenBwd) {
+            *reinterpret_cast<float4*>(p.out[1] + (to - p.out[0]) + i) =
+                make_float4(dg[0], dg[1], dg[2], dg[3]);
+            *reinterpret_cast<float4*>(p.out[2] + (to - p.out[0]) + i) =
+                make_float4(du[0], du[1], du[2], du[3]);
+          }
         }
       }
     } else {
-      wait(&sums, 0);
-      tc_fence_after();
-      const int64_t r = m0 + row;
-      if constexpr (kHid) {
+      const int width = static_cast<int>(p.out_ld), c = n0 + 32 * part;
+      if (r < p.rows) {
+        float* to = p.out[0] + r * p.out_ld + c;
 #pragma unroll
-        for (int c = half * 32; c < half * 32 + 32; c += 16) {
-          if (n0 + c >= p.h) break;
-          float g[16], u[16], dh[16];
-          tmem_ld(acc + quarter + c, g);
-          tmem_ld(acc + quarter + 64 + c, u);
-          if constexpr (kJob == kHiddenBwd) tmem_ld(acc + quarter + 128 + c, dh);
-          tmem_wait_ld(g);
-          tmem_wait_ld(u);
-          if constexpr (kJob == kHiddenBwd) tmem_wait_ld(dh);
-          if (r < p.rows) {
-            float* to = p.out[0] + r * p.out_ld + n0 + c;
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              float h[4], dg[4], du[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float x = g[i + k], s = __fdividef(1.f, 1.f + __expf(-x)), act = x * s;
-                h[k] = act * u[i + k];
-                if constexpr (kJob == kHiddenBwd) {
-                  dg[k] = dh[i + k] * u[i + k] * (s + act * (1.f - s));
-                  du[k] = dh[i + k] * act;
-                }
-              }
-              *reinterpret_cast<float4*>(to + i) = make_float4(h[0], h[1], h[2], h[3]);
-              if constexpr (kJob == kHiddenBwd) {
-                *reinterpret_cast<float4*>(p.out[1] + (to - p.out[0]) + i) =
-                    make_float4(dg[0], dg[1], dg[2], dg[3]);
-                *reinterpret_cast<float4*>(p.out[2] + (to - p.out[0]) + i) =
-                    make_float4(du[0], du[1], du[2], du[3]);
-              }
-            }
-          }
-          __syncwarp();
-        }
-      } else {
-        const int width = static_cast<int>(p.out_ld);
-        for (int c = half * 16; c < n; c += 32) {
-          float v[16];
-          tmem_ld(acc + quarter + c, v);
-          tmem_wait_ld(v);
-          if (r < p.rows) {
-            float* to = p.out[0] + r * p.out_ld + n0 + c;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n0 + c + i < width) to[i] = v[i];
-          }
-          __syncwarp();
-        }
+        for (int i = 0; i < 32; ++i)
+          if (c + i < width) to[i] = sum[i >> 4][i & 15];
       }
     }
   } else {
-    const bool on = elect_one();
     // Parts of A and B, the smallest products first.
     constexpr int kPa[6] = {0, 1, 2, 0, 1, 0}, kPb[6] = {2, 1, 0, 1, 0, 0};
-    int term = which, k0 = 0, fresh = 1, drains = 0;
+    int term = which, k0 = 0;
     for (int s = 0; s < total; ++s) {
       const int st = s & 1;
+      if (s >= 2) wait(&drained[st], (s >> 1) - 1);
       wait(&full[st], s >> 1);
-      if (kMn && fresh && drains > 0) wait(&drained, drains - 1);
       tc_fence_after();
       const uint32_t from = base + (p.stages == 2 ? st : 0) * kStage;
       const bool b_mn = kMn || (kJob == kHiddenBwd ? term == 1 : kJob == kOutput && p.d > 0);
       const int k = kMn ? kStep : p.t[term].k;
       const int steps = kMn ? 4 : min(4, (k - k0 + 15) >> 4);
-      const bool second = kJob == kHiddenBwd && term == 1;
-      const uint32_t to = acc + (second ? 128 : 0);
-      const uint32_t id = tc_idesc(second ? 64 : n, kMn, b_mn);
+      const uint32_t to = acc + st * 128;
+      const uint32_t id = tc_idesc(kJob == kHiddenBwd && term == 1 ? 64 : n, kMn, b_mn);
+      const uint32_t da = kMn ? desc_mn(from, kPart / 2) : desc_k(from);
+      const uint32_t db = b_mn ? desc_mn(from + 3 * kPart, kPart / 2) : desc_k(from + 3 * kPart);
+      const uint32_t sa = kMn ? kStepMn : kStepK, sb = b_mn ? kStepMn : kStepK;
 #pragma unroll
-      for (int q = 0; q < 6; ++q) {
-        const uint32_t pa = from + kPa[q] * kPart, pb = from + (3 + kPb[q]) * kPart;
-        const uint32_t da = kMn ? desc_mn(pa, kPart / 2) : desc_k(pa);
-        const uint32_t db = b_mn ? desc_mn(pb, kPart / 2) : desc_k(pb);
-        if (on) {
-          for (int i = 0; i < steps; ++i)
-            tc_mma(to, da + i * (kMn ? kStepMn : kStepK), db + i * (b_mn ? kStepMn : kStepK), id,
-                   !(fresh && q == 0 && i == 0));
-        }
-        __syncwarp();
-      }
-      fresh = 0;
-      tc_commit(&empty[st]);
-      if constexpr (kMn) {
-        if ((s + 1) % kSums == 0 || s + 1 == total) {
-          tc_commit(&sums);
-          fresh = 1, ++drains;
-        }
-      } else {
-        k0 += kStep;
-        if (k0 >= k) {
-          k0 = 0, ++term;
-          if (kJob == kHiddenBwd) fresh = 1;  // the other accumulators
-        }
-      }
+      for (int q = 0; q < 6; ++q)
+        tc_mma_steps<4>(to, da + kPa[q] * (kPart >> 4), sa, db + kPb[q] * (kPart >> 4), sb, id, steps,
+                        q > 0);
+      tc_commit(&done[st]);
+      if (!kMn && (k0 += kStep) >= k) k0 = 0, ++term;
     }
-    if (!kMn) {
-      tc_commit(&sums);
-      wait(&sums, 0);
-    }
+    if (total > 0) wait(&done[(total - 1) & 1], (total - 1) >> 1);
   }
   __syncwarp();
   tc_fence_before();
@@ -371,7 +339,7 @@ template <int kJob>
 int launch32(Tc32Params p, dim3 grid, cudaStream_t s) {
   int total = kJob == kWeights ? 2 : 0;
   for (int t = 0; kJob != kWeights && t < p.terms; ++t) total += ceil_div(p.t[t].k, kStep);
-  p.stages = total > 1 ? 2 : 1;  // one stage leaves room for two blocks to an SM
+  p.stages = total > 1 ? 2 : 1;
   const int smem = p.stages * kStage + 1024;
   TGS_CUDA(cudaFuncSetAttribute(ffn_tc32_kernel<kJob>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 smem));
@@ -380,11 +348,12 @@ int launch32(Tc32Params p, dim3 grid, cudaStream_t s) {
   return TGS_OK;
 }
 
-// Rows of a batch: its three hidden matrices together take about 64 MB of the
-// 126 MB of L2.
+// Rows of a batch: its three hidden matrices together take at most about 64 MB
+// of the 126 MB of L2; batches of one size.
 int64_t batch_rows(int64_t n, int h) {
-  const int64_t rows = (16ll << 20) / (3 * ceil_div(h, 64) * 64) / kTile * kTile;
-  return std::min<int64_t>(ceil_div<int64_t>(n, kTile) * kTile, std::max<int64_t>(rows, kTile));
+  const int64_t tiles = ceil_div<int64_t>(n, kTile);
+  const int64_t most = std::max<int64_t>(1, (16ll << 20) / (3 * ceil_div(h, 64) * 64) / kTile);
+  return ceil_div(tiles, ceil_div(tiles, most)) * kTile;
 }
 
 int64_t padded(int h) { return ceil_div(h, 64) * 64; }
