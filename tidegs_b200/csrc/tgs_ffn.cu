@@ -492,11 +492,8 @@ extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32
                                           int32_t backward) {
   if (n <= 0 || d <= 0 || h <= 0 || o <= 0) return 0;
   if (dtype != TGS_F32) return ffn_tc_scratch_floats(n, d, h, o, backward != 0);
-  const bool large = large_f32(n, d, h, o);
-  if (!backward) return large ? tc32_hidden_floats(n, h, false) : 0;
-  if (!large) return weights_floats(n, d, h, o);
-  return ceil_div<int64_t>(tc32_slices(n, d, h, o) * static_cast<int64_t>(h) * (2 * d + o), 4) * 4 +
-         tc32_hidden_floats(n, h, true);
+  if (large_f32(n, d, h, o)) return tc32_scratch_floats(n, d, h, o, backward != 0);
+  return backward ? weights_floats(n, d, h, o) : 0;
 }
 
 extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {

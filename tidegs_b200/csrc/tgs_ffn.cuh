@@ -26,6 +26,6 @@ int ffn_tc_backward(const FfnParams& p, cudaStream_t s);
 // the start of the scratch.
 int ffn_tc32_run(const FfnParams& p, bool backward, cudaStream_t s);
 int tc32_slices(int64_t n, int d, int h, int o);
-int64_t tc32_hidden_floats(int64_t n, int h, bool backward);
+int64_t tc32_scratch_floats(int64_t n, int d, int h, int o, bool backward);
 
 }  // namespace tgs
