@@ -5,10 +5,9 @@
 //   dX = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X, dWd = dY^T H.
 // The hidden values stay on chip: the backward recomputes G and U.
 //
-// This file: the entry points, and 32-bit tensors, whose products run on the
-// ordinary fp32 pipes (a 32-bit product takes six bf16 products on the tensor
-// cores, and the operands' three parts do not fit beside one another in shared
-// memory). bf16 tensors take the tensor cores (tgs_ffn_tc.cu).
+// This file: the entry points, and narrow blocks of 32-bit tensors, whose
+// products run on the ordinary fp32 pipes. bf16 tensors take the tensor cores
+// (tgs_ffn_tc.cu), and wide blocks of 32-bit tensors too (tgs_ffn_tc32.cu).
 //
 // A block of 256 threads, 16 x 16, works on a tile of 16 kR rows and chunks of
 // 32 hidden values. Everything lies in shared memory with the contracted index
@@ -429,10 +428,14 @@ int launch_weights(const FfnParams& p, int slices, cudaStream_t s) {
   return TGS_OK;
 }
 
-// Whether a 32-bit call takes the tensor cores.
-bool large_f32(int64_t n, int d, int h, int o) {
-  (void)d, (void)h, (void)o;
-  return n >= 4096;
+// Whether a 32-bit call takes the tensor cores: by the multiply-adds of a row.
+// Their fixed work on each matrix (splitting, a trip through L2) pays for
+// itself from about 12,000 on, at any number of rows. 100,000 rows, forward and
+// forward + backward, fp32 pipes against tensor cores: 35 -> 96 -> 3 (7,008) 63
+// and 397 us against 119 and 507; 48 -> 96 -> 48 (13,824) 99 and 617 against
+// 129 and 493; 128 -> 256 -> 128 (98,304) 807 and 4127 against 300 and 1207.
+bool wide_f32(int d, int h, int o) {
+  return static_cast<int64_t>(h) * (2 * d + o) >= 12288;
 }
 
 int sum_slices(const FfnParams& p, int slices, cudaStream_t s) {
@@ -443,7 +446,7 @@ int sum_slices(const FfnParams& p, int slices, cudaStream_t s) {
 }
 
 int ffn_backward_f32(const FfnParams& p, cudaStream_t s) {
-  if (large_f32(p.n, p.d, p.h, p.o)) {
+  if (wide_f32(p.d, p.h, p.o)) {
     if (int rc = ffn_tc32_run(p, true, s)) return rc;
     return p.dwg ? sum_slices(p, tc32_slices(p.n, p.d, p.h, p.o), s) : TGS_OK;
   }
@@ -492,7 +495,7 @@ extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32
                                           int32_t backward) {
   if (n <= 0 || d <= 0 || h <= 0 || o <= 0) return 0;
   if (dtype != TGS_F32) return ffn_tc_scratch_floats(n, d, h, o, backward != 0);
-  if (large_f32(n, d, h, o)) return tc32_scratch_floats(n, d, h, o, backward != 0);
+  if (wide_f32(d, h, o)) return tc32_scratch_floats(n, d, h, o, backward != 0);
   return backward ? weights_floats(n, d, h, o) : 0;
 }
 
@@ -505,7 +508,7 @@ extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
   const FfnParams p = ffn_params(*a);
   cudaStream_t s = as_stream(stream);
   if (a->dtype == TGS_BF16) return ffn_tc_forward(p, s);
-  return large_f32(p.n, p.d, p.h, p.o) ? ffn_tc32_run(p, false, s) : rows_f32<false>(p, s);
+  return wide_f32(p.d, p.h, p.o) ? ffn_tc32_run(p, false, s) : rows_f32<false>(p, s);
 }
 
 extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {

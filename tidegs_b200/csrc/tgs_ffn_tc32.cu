@@ -1,4 +1,4 @@
-// Gated feed-forward block in 32 bits on the tensor cores, for large calls; the
+// Gated feed-forward block in 32 bits on the tensor cores, for wide blocks; the
 // formulas stand in tgs_ffn.cu.
 //
 // A 32-bit number is the sum of three bf16 numbers up to 2^-24 of it (8 bits
@@ -289,16 +289,30 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
               du[i] = d * act;
             }
           }
-          const int64_t at = (static_cast<int64_t>(tile.m) * p.h.col_blocks + tile.n0) * kBlock3 +
-                             unit_offset(row, 4 * half + 2 * q + u8);
-          auto put = [&](const Split& to, const float (&v)[8]) {
+          // The stages' memory is free now: the blocks are put together there
+          // (16-byte stores to global memory took four fifths of the kernel).
+          const uint32_t at = base + unit_offset(row, 4 * half + 2 * q + u8);
+          auto put = [&](int matrix, const float (&v)[8]) {
             split8(v, [&](int part, uint4 w) {
-              *reinterpret_cast<uint4*>(to.p + at + part * kPart) = w;
+              st_shared16(at + matrix * kBlock3 + part * kPart, w);
             });
           };
-          put(p.h, h);
-          if constexpr (kJob == kHiddenBwd) put(p.dg, dg), put(p.du, du);
+          put(0, h);
+          if constexpr (kJob == kHiddenBwd) put(1, dg), put(2, du);
         }
+      }
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, %0;" ::"n"(kAdders) : "memory");
+      if (threadIdx.x == 0) {
+        const int64_t block = (static_cast<int64_t>(tile.m) * p.h.col_blocks + tile.n0) * kBlock3;
+        const uint8_t* from = raw + (base - smem_addr(raw));
+        bulk_s2g(p.h.p + block, from, kBlock3);
+        if constexpr (kJob == kHiddenBwd) {
+          bulk_s2g(p.dg.p + block, from + kBlock3, kBlock3);
+          bulk_s2g(p.du.p + block, from + 2 * kBlock3, kBlock3);
+        }
+        bulk_commit();
+        bulk_wait_all();
       }
     } else {
       float* to;
@@ -316,7 +330,12 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
       }
       const int c0 = tile.n0 * kTile + 64 * half;
       if (on) {
-        const bool vec = fresh && width % 4 == 0 && aligned16(p.out);
+        if (!fresh) {  // all loads before the first store
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (c0 + i < width) sum[i >> 4][i & 15] += to[c0 + i];
+        }
+        const bool vec = width % 4 == 0 && aligned16(p.out);
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {
           const float* v = &sum[i >> 4][i & 15];
@@ -325,7 +344,7 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (c0 + i + k < width) to[c0 + i + k] = fresh ? v[k] : to[c0 + i + k] + v[k];
+              if (c0 + i + k < width) to[c0 + i + k] = v[k];
           }
         }
       }
