@@ -835,6 +835,12 @@ typedef struct {
 /* Gradients of the layer norm; the row statistics are recomputed from x. */
 TGS_API int tgs_layer_norm_bwd(const TgsLayerNormBwdArgs* args, void* stream);
 
+/* Rows of 16-bit values at any stride and alignment -> rows of
+ * ceil(c / 8) * 8 values at dst (16-byte aligned, contiguous), zeros at their
+ * ends: what the entry points below take of bf16 matrices. */
+TGS_API int tgs_align_rows(const void* src, int64_t stride, int64_t n, int32_t c, void* dst,
+                           void* stream);
+
 typedef struct {
   const void* x;       /* [n, d] */
   const void* w_gate;  /* [h, d] contiguous */
@@ -842,7 +848,8 @@ typedef struct {
   const void* w_down;  /* [o, h] contiguous */
   void* y;             /* [n, o] contiguous (forward) */
   int64_t n;           /* at most 2^31 */
-  int64_t x_stride;    /* elements from row to row, >= d */
+  int64_t x_stride;    /* elements from row to row, >= d; of bf16 matrices a
+                          multiple of 8, x 16-byte aligned (v_y too) */
   int32_t d;           /* 1..256 */
   int32_t h;           /* 1..4096 */
   int32_t o;           /* 1..256 */

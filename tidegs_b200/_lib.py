@@ -291,6 +291,7 @@ SIGNATURES = {
     "tgs_layer_norm_fwd": (C.c_int, [C.POINTER(LayerNormArgs), _vp]),
     "tgs_layer_norm_scratch_floats": (_i64, [_i64, _i32]),
     "tgs_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormBwdArgs), _vp]),
+    "tgs_align_rows": (C.c_int, [_vp, _i64, _i64, _i32, _vp, _vp]),
     "tgs_ffn_fwd": (C.c_int, [C.POINTER(FfnArgs), _vp]),
     "tgs_ffn_scratch_floats": (_i64, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "tgs_ffn_bwd": (C.c_int, [C.POINTER(FfnBwdArgs), _vp]),
@@ -351,7 +352,7 @@ KERNELS_PER_CALL = {
     # the library version and are not counted here)
     "tgs_isect_depth_order": 1, "tgs_isect_sort_tiles": 0,
     "tgs_layer_norm_fwd": 1, "tgs_layer_norm_bwd": 2, "tgs_ffn_fwd": 1, "tgs_ffn_bwd": 2,
-    "tgs_dropout": 1,
+    "tgs_dropout": 1, "tgs_align_rows": 1,
 }
 launch_counter = {"kernels": 0}
 

@@ -194,12 +194,31 @@ def check(device=None) -> None:
         raise RuntimeError(f"[gated_feed_forward] {problem}")
 
 
+def _ffn_rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """_rows, for bfloat16 with every row on a 16-byte boundary."""
+    t = _rows(t, width)
+    if t.dtype is not torch.bfloat16 or t.shape[0] == 0:
+        return t
+    if t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or t.stride(0) % 8 == 0):
+        return t
+    out = torch.empty((t.shape[0], -(-width // 8) * 8), dtype=t.dtype, device=t.device)
+    with _on(t.device):
+        _lib.call("tgs_align_rows", t.data_ptr(), _row_stride(t), t.shape[0], width, out.data_ptr(),
+                  _stream(t.device))
+    return out[:, :width]
+
+
+def _ffn_stride(t: torch.Tensor) -> int:
+    n, width = t.shape
+    return t.stride(0) if n > 1 else -(-width // 8) * 8
+
+
 def _ffn_args(x, w_gate, w_up, w_down, backward: bool):
     """(arguments, scratch tensor or None); on the tensors' device."""
     a = _lib.FfnArgs()
     a.x, a.w_gate = x.data_ptr(), w_gate.data_ptr()
     a.w_up, a.w_down = w_up.data_ptr(), w_down.data_ptr()
-    a.n, a.x_stride = int(x.shape[0]), _row_stride(x)
+    a.n, a.x_stride = x.shape[0], _ffn_stride(x)
     a.d, a.h, a.o = int(w_gate.shape[1]), int(w_gate.shape[0]), int(w_down.shape[0])
     a.dtype = _lib.DTYPES[x.dtype]
     a.err = _lib.ptr(_err_word(x.device))
@@ -210,7 +229,7 @@ def _ffn_args(x, w_gate, w_up, w_down, backward: bool):
 
 
 def _ffn_forward(x, w_gate, w_up, w_down):
-    rows = _rows(x, x.shape[-1])
+    rows = _ffn_rows(x, x.shape[-1])
     weights = [w.contiguous() for w in (w_gate, w_up, w_down)]
     y = torch.empty((*x.shape[:-1], w_down.shape[0]), dtype=x.dtype, device=x.device)
     with _on(x.device):
@@ -233,11 +252,11 @@ class _GatedFeedForward(torch.autograd.Function):
         weights = [w.contiguous() for w in weights]
         need_x, *need_w = ctx.needs_input_grad
         d, o = x.shape[-1], weights[2].shape[0]
-        rows, v_rows = _rows(x, d), _rows(v_y, o)
+        rows, v_rows = _ffn_rows(x, d), _ffn_rows(v_y, o)
         v_x = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
         v_w = [torch.empty_like(w) for w in weights] if any(need_w) else [None] * 3
         b = _lib.FfnBwdArgs()
-        b.v_y, b.v_y_stride, b.v_x = v_rows.data_ptr(), _row_stride(v_rows), _lib.ptr(v_x)
+        b.v_y, b.v_y_stride, b.v_x = v_rows.data_ptr(), _ffn_stride(v_rows), _lib.ptr(v_x)
         b.v_w_gate, b.v_w_up, b.v_w_down = (_lib.ptr(v) for v in v_w)
         with _on(x.device):
             b.fwd, _scratch = _ffn_args(rows, *weights, backward=True)

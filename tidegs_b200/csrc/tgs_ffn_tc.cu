@@ -13,7 +13,7 @@
 //                next chunk's first products do not wait behind the output)
 //   warp  18     weight blocks (bulk copies)
 //   warp  19     row tiles by tensor-map copies
-//   warps 20-23  the output tile; row tiles that no tensor map describes
+//   warps 20-23  the output tile
 // The same block of weights serves both products: as K-major operand of one
 // and as MN-major operand of the other.
 //
@@ -29,8 +29,8 @@ namespace tgs {
 namespace {
 
 constexpr int kEpi = 512;      // activation threads, in two groups
-constexpr int kLoad = 128;     // threads of the output, and of rows that no tensor map describes
-constexpr int kTcThreads = kEpi + 128 + kLoad;
+constexpr int kOut = 128;      // threads of the output
+constexpr int kTcThreads = kEpi + 128 + kOut;
 constexpr int kWarpF = kEpi / 32, kWarpS = kWarpF + 1, kWarpW = kWarpF + 2, kWarpT = kWarpF + 3;
 constexpr int kTile = 128;     // rows
 constexpr int kChunk = 64;     // hidden values
@@ -49,7 +49,7 @@ struct TcParams {
   int kd, ko;      // 16-steps of D and O
   int nx, nh, nb, ny, slots, slots_f;  // buffers: row tiles, hidden, first and output accumulators
   int ycols;                  // columns of one output accumulator
-  int resident, tma_x, tma_dy, vec_y;
+  int resident, vec_y;
   uint32_t tile_bytes, h_bytes, w_bytes;
   uint32_t tmem_cols;
   // Block b takes chunks [cpc g, cpc g + cpc) of tiles s, s + slices, ... with
@@ -132,6 +132,26 @@ __global__ void __launch_bounds__(256) ffn_pack_kernel(const TcParams p, uint8_t
   uint32_t at;
   const uint4 v = weight_unit(p, 0, p.nc, e, &at);
   *reinterpret_cast<uint4*>(dst + at) = v;
+}
+
+// Rows of 16-bit values to rows of whole 16-byte units, zeros at their ends.
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restrict__ src,
+                                                         int64_t stride, int64_t n, int c,
+                                                         uint4* __restrict__ dst, int units) {
+  const int64_t all = n * units;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < all;
+       e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = e / units;
+    const int col = static_cast<int>(e - row * units) * 8;
+    const uint16_t* s = src + row * stride + col;
+    union {
+      uint4 q;
+      uint16_t t[8];
+    } u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u.t[i] = col + i < c ? s[i] : 0;
+    dst[e] = u.q;
+  }
 }
 
 // --- waits -----------------------------------------------------------------------
@@ -226,29 +246,6 @@ __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint
                 make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
 }
 
-// A row tile -> operand blocks, by threads: for matrices that no tensor map
-// can describe. As many neighbouring threads to a row as it has 16-byte units
-// in the block (a power of two), so that narrow rows go many at a time.
-__device__ __forceinline__ void load_tile(uint32_t dst, const __nv_bfloat16* src, int64_t stride,
-                                          int64_t r0, int64_t n, int cols, int k16, int tid) {
-  for (int c = 0; 4 * c < k16; ++c) {
-    const int left_units = 2 * k16 - 8 * c;
-    const int per_row = left_units > 4 ? 8 : left_units > 2 ? 4 : 2;
-    const int unit = tid & (per_row - 1), rows = kLoad / per_row;
-    if (unit >= left_units) continue;
-    const int col = c * kBlockCols + unit * 8;
-    int row = tid / per_row;
-    const __nv_bfloat16* from = src + (r0 + row) * stride + col;
-    int64_t left = n - r0 - row;
-#pragma unroll 4
-    for (int i = 0; i < per_row; ++i) {
-      st_shared16(dst + c * kBlockBytes + unit_offset(row, unit),
-                  left > 0 ? load_unit(from, 0, cols - col, false) : make_uint4(0, 0, 0, 0));
-      row += rows, from += rows * stride, left -= rows;
-    }
-  }
-}
-
 __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, int64_t tile,
                                              int out, int lane_row) {
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.f.y);
@@ -330,11 +327,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
   if (warp == kWarpF) {
     tmem_alloc(&bars.tmem, p.tmem_cols);
     if (lane == 0) {
-      const int arrivals = 1 + (!p.tma_x || (kBwd && !p.tma_dy) ? kLoad / 32 : 0);
-      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], arrivals), mbar_init(&bars.xempty[i], 1);
+      for (int i = 0; i < kMaxTiles; ++i) mbar_init(&bars.xfull[i], 1), mbar_init(&bars.xempty[i], 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars.gfull[i], 1), mbar_init(&bars.gempty[i], kEpi / 64);
-        mbar_init(&bars.yfull[i], 1), mbar_init(&bars.yempty[i], kLoad / 32);
+        mbar_init(&bars.yfull[i], 1), mbar_init(&bars.yempty[i], kOut / 32);
       }
       for (int i = 0; i < kMaxHid; ++i) mbar_init(&bars.hfull[i], kEpi / 64), mbar_init(&bars.hempty[i], 1);
       mbar_init(&bars.done, 2), mbar_init(&bars.accfull, 1);
@@ -585,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
         if (!wait.ok) break;
         const int64_t r0 = (slice + static_cast<int64_t>(t) * p.slices) * kTile;
         const uint32_t dst = xs + xb * p.tile_bytes;
-        const int xblocks = p.tma_x ? p.cd : 0, yblocks = kBwd && p.tma_dy ? p.co : 0;
+        const int xblocks = p.cd, yblocks = kBwd ? p.co : 0;
         mbar_arrive_expect_tx(&bars.xfull[xb], (xblocks + yblocks) * kBlockBytes);
         for (int c = 0; c < xblocks; ++c)
           tma_load_2d(dst + c * kBlockBytes, &p.xmap, c * kBlockCols, static_cast<int>(r0),
@@ -603,37 +599,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
       }
     }
   } else {
-    const bool tx = !p.tma_x, ty = kBwd && !p.tma_dy;
-    const int tid = threadIdx.x - kEpi - 128;
-    const int out = kBwd ? p.f.d : p.f.o;
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;
-    auto row_of = [&](int t) { return (slice + static_cast<int64_t>(t) * p.slices) * kTile; };
-    int xb = 0, round = 0;
-    // Loads run nx tiles ahead of the output: the buffer that a load waits for
-    // is then never one whose tile waits for this output.
-    const int ahead = tx || ty ? p.nx : 0;
-    for (int t = 0; t < mine + ahead; ++t) {
-      if (ahead && t < mine) {
-        if (round > 0) wait(&bars.xempty[xb], round - 1);
-        const uint32_t dst = xs + xb * p.tile_bytes;
-        if (tx)
-          load_tile(dst, static_cast<const __nv_bfloat16*>(p.f.x), p.f.x_stride, row_of(t), p.f.n,
-                    p.f.d, p.kd, tid);
-        if (ty)
-          load_tile(dst + p.cd * kBlockBytes, static_cast<const __nv_bfloat16*>(p.f.dy),
-                    p.f.dy_stride, row_of(t), p.f.n, p.f.o, p.ko, tid);
-        fence_proxy_async_smem();
-        warp_arrive(&bars.xfull[xb], lane);
-        if (++xb == p.nx) xb = 0, ++round;
-      }
-      const int done = t - ahead;
-      if (kRows && done >= 0) {
-        wait(&bars.yfull[done & 1], done >> 1);
+    if constexpr (kRows) {
+      const int out = kBwd ? p.f.d : p.f.o;
+      for (int t = 0; t < mine; ++t) {
+        wait(&bars.yfull[t & 1], t >> 1);
         tc_fence_after();
-        store_output(p, yacc + (p.ny == 2 ? done & 1 : 0) * p.ycols + quarter,
-                     row_of(done) / kTile, out, (warp & 3) * 32 + lane);
+        store_output(p, yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols + quarter,
+                     slice + static_cast<int64_t>(t) * p.slices, out, (warp & 3) * 32 + lane);
         tc_fence_before();
-        warp_arrive(&bars.yempty[done & 1], lane);
+        warp_arrive(&bars.yempty[t & 1], lane);
       }
     }
     if constexpr (kHasDw) {
@@ -721,15 +696,10 @@ TcParams tc_params(const FfnParams& f) {
   return p;
 }
 
-// Tensor maps for the matrices that have one; threads load the others.
 int make_maps(TcParams& p, bool bwd) {
   const FfnParams& f = p.f;
-  p.tma_x = f.x_stride % 8 == 0 && aligned16(f.x);
-  p.tma_dy = bwd && f.dy_stride % 8 == 0 && aligned16(f.dy);
-  if (p.tma_x) {
-    if (int rc = make_row_map(&p.xmap, f.x, f.n, f.d, f.x_stride)) return rc;
-  }
-  return p.tma_dy ? make_row_map(&p.dymap, f.dy, f.n, f.o, f.dy_stride) : TGS_OK;
+  if (int rc = make_row_map(&p.xmap, f.x, f.n, f.d, f.x_stride)) return rc;
+  return bwd ? make_row_map(&p.dymap, f.dy, f.n, f.o, f.dy_stride) : TGS_OK;
 }
 
 // Buffers for Y or dX. Shared memory goes first to the weights (as a
@@ -931,3 +901,20 @@ int ffn_tc_backward(const FfnParams& f, cudaStream_t s) {
 }
 
 }  // namespace tgs
+
+extern "C" int tgs_align_rows(const void* src, int64_t stride, int64_t n, int32_t c, void* dst,
+                              void* stream) {
+  using namespace tgs;
+  TGS_CHECK_ARG(n >= 0 && c >= 1, "tgs_align_rows: bad sizes (n %lld, c %d)", static_cast<long long>(n),
+                c);
+  if (n == 0) return TGS_OK;
+  TGS_CHECK_ARG(src && dst && aligned16(dst), "tgs_align_rows: NULL or unaligned pointer");
+  TGS_CHECK_ARG(n == 1 || stride >= c, "tgs_align_rows: rows overlap (stride %lld, c %d)",
+                static_cast<long long>(stride), c);
+  const int units = ceil_div(c, 8);
+  const int64_t blocks = std::min<int64_t>(ceil_div<int64_t>(n * units, 256), sm_count() * 16ll);
+  align_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, as_stream(stream)>>>(
+      static_cast<const uint16_t*>(src), stride, n, c, static_cast<uint4*>(dst), units);
+  TGS_LAUNCH_CHECK();
+  return TGS_OK;
+}
