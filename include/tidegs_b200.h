@@ -846,7 +846,7 @@ typedef struct {
   const void* w_gate;  /* [h, d] contiguous */
   const void* w_up;    /* [h, d] contiguous */
   const void* w_down;  /* [o, h] contiguous */
-  void* y;             /* [n, o] contiguous (forward) */
+  void* y;             /* [n, o] contiguous, 16-byte aligned (forward) */
   int64_t n;           /* at most 2^31 */
   int64_t x_stride;    /* elements from row to row, >= d; of bf16 matrices a
                           multiple of 8, x 16-byte aligned (v_y too) */
@@ -870,7 +870,7 @@ typedef struct {
   TgsFfnArgs fwd;      /* y unused */
   const void* v_y;     /* [n, o] */
   int64_t v_y_stride;
-  void* v_x;           /* [n, d] contiguous, or NULL */
+  void* v_x;           /* [n, d] contiguous, 16-byte aligned, or NULL */
   void* v_w_gate;      /* the three weights' gradients: all or none */
   void* v_w_up;
   void* v_w_down;

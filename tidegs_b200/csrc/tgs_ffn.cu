@@ -507,8 +507,8 @@ extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
   if (int rc = check_ffn(a, "tgs_ffn_fwd")) return rc;
   if (a->n == 0) return TGS_OK;
   TGS_CHECK_ARG(a->y != nullptr, "tgs_ffn_fwd: NULL pointer");
-  TGS_CHECK_ARG(aligned_rows(*a, a->x, a->x_stride),
-                "tgs_ffn_fwd: rows of x are not 16-byte aligned (stride %lld)",
+  TGS_CHECK_ARG(aligned_rows(*a, a->x, a->x_stride) && aligned16(a->y) && aligned16(a->scratch),
+                "tgs_ffn_fwd: y, scratch or the rows of x are not 16-byte aligned (stride %lld)",
                 static_cast<long long>(a->x_stride));
   TGS_CHECK_ARG(a->scratch || !tgs_ffn_scratch_floats(a->n, a->d, a->h, a->o, a->dtype, 0),
                 "tgs_ffn_fwd: scratch is NULL");
@@ -527,8 +527,9 @@ extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {
                 "tgs_ffn_bwd: the weights' gradients are all given or none");
   TGS_CHECK_ARG(a.n == 0 || (b->v_y && (b->v_x || weights)), "tgs_ffn_bwd: NULL pointer");
   TGS_CHECK_ARG(a.n <= 1 || b->v_y_stride >= a.o, "tgs_ffn_bwd: rows of v_y overlap");
-  TGS_CHECK_ARG(aligned_rows(a, a.x, a.x_stride) && aligned_rows(a, b->v_y, b->v_y_stride),
-                "tgs_ffn_bwd: rows of x or v_y are not 16-byte aligned (strides %lld, %lld)",
+  TGS_CHECK_ARG(aligned_rows(a, a.x, a.x_stride) && aligned_rows(a, b->v_y, b->v_y_stride) &&
+                    aligned16(b->v_x) && aligned16(a.scratch),
+                "tgs_ffn_bwd: v_x, scratch or the rows of x or v_y are not 16-byte aligned (strides %lld, %lld)",
                 static_cast<long long>(a.x_stride), static_cast<long long>(b->v_y_stride));
   TGS_CHECK_ARG(a.scratch || !tgs_ffn_scratch_floats(a.n, a.d, a.h, a.o, a.dtype, 1),
                 "tgs_ffn_bwd: scratch is NULL");

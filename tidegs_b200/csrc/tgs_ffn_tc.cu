@@ -50,7 +50,7 @@ struct TcParams {
   int nx, nh, nb, ny, slots, slots_f;  // buffers: row tiles, hidden, first and output accumulators
   int ycols;                  // columns of one output accumulator
   int resident, vec_y;
-  uint32_t tile_bytes, h_bytes, w_bytes;
+  uint32_t tile_bytes, h_bytes, w_bytes, stage_bytes;
   uint32_t tmem_cols;
   // Block b takes chunks [cpc g, cpc g + cpc) of tiles s, s + slices, ... with
   // g = b % groups and s = b / groups. With `split`, odd g are the blocks of
@@ -246,8 +246,13 @@ __device__ __forceinline__ void store_granule(uint32_t block, uint32_t row, uint
                 make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
 }
 
+// The output tile's row `lane_row`, out of its accumulators. A tile of the
+// output is one piece of memory that starts on a 16-byte boundary; where its
+// rows do not, it is put together at `stage` and stored as a whole (2-byte
+// stores of rows of 59 took three times the kernel's other work). `stage` 0:
+// the rows are stored apart (aligned ones, or no room).
 __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, int64_t tile,
-                                             int out, int lane_row) {
+                                             int out, int lane_row, uint32_t stage) {
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(p.f.y);
   const int64_t row = tile * kTile + lane_row;
   for (int c = 0; c < out; c += 16) {
@@ -255,7 +260,14 @@ __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, in
     tmem_ld(acc + c, v);
     tmem_wait_ld(v);
     __nv_bfloat16* dst = y + row * out + c;
-    if (row >= p.f.n) {
+    if (stage) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < out)
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(stage + 2 * (lane_row * out + c + i)),
+                       "h"(__bfloat16_as_ushort(__float2bfloat16_rn(v[i])))
+                       : "memory");
+    } else if (row >= p.f.n) {
     } else if (p.vec_y) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -275,6 +287,20 @@ __device__ __forceinline__ void store_output(const TcParams& p, uint32_t acc, in
     }
     __syncwarp();  // the next load is the whole warp's
   }
+}
+
+// The staged tile, by the output's threads.
+__device__ __forceinline__ void store_staged(const TcParams& p, int64_t tile, int out,
+                                             const uint8_t* stage, int tid) {
+  asm volatile("bar.sync 1, %0;" ::"n"(kOut) : "memory");
+  const int64_t left = p.f.n - tile * kTile;
+  const int bytes = static_cast<int>(left < kTile ? left : kTile) * out * 2;
+  uint8_t* y = static_cast<uint8_t*>(p.f.y) + tile * kTile * out * 2;
+  for (int e = tid; e < bytes / 16; e += kOut)
+    reinterpret_cast<uint4*>(y)[e] = reinterpret_cast<const uint4*>(stage)[e];
+  for (int e = (bytes & ~15) / 2 + tid; e < bytes / 2; e += kOut)
+    reinterpret_cast<uint16_t*>(y)[e] = reinterpret_cast<const uint16_t*>(stage)[e];
+  asm volatile("bar.sync 1, %0;" ::"n"(kOut) : "memory");
 }
 
 // This block's sum of one weight gradient's chunk, out of its accumulators.
@@ -307,6 +333,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
   const uint32_t xs = base;                             // nx tiles: X blocks, then dY blocks
   const uint32_t hs = xs + p.nx * p.tile_bytes;         // nh hidden buffers
   const uint32_t ws = hs + p.nh * p.h_bytes;            // weights, or the ring
+  const uint32_t ys = ws + (p.resident ? p.w_bytes : p.slots * kBlockBytes);  // staged output
   // from lane 0, so that the compiler sees the roles' branches as uniform
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr bool kBwd = kMode != kFwd, kHasDw = kMode >= kDw, kRows = kMode != kDw;
@@ -606,9 +633,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
         wait(&bars.yfull[t & 1], t >> 1);
         tc_fence_after();
         store_output(p, yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols + quarter,
-                     slice + static_cast<int64_t>(t) * p.slices, out, (warp & 3) * 32 + lane);
+                     slice + static_cast<int64_t>(t) * p.slices, out, (warp & 3) * 32 + lane,
+                     p.stage_bytes ? ys : 0);
         tc_fence_before();
         warp_arrive(&bars.yempty[t & 1], lane);
+        if (p.stage_bytes)
+          store_staged(p, slice + static_cast<int64_t>(t) * p.slices, out, raw + (ys - smem_addr(raw)),
+                       (warp & 3) * 32 + lane);
       }
     }
     if constexpr (kHasDw) {
@@ -702,6 +733,13 @@ int make_maps(TcParams& p, bool bwd) {
   return bwd ? make_row_map(&p.dymap, f.dy, f.n, f.o, f.dy_stride) : TGS_OK;
 }
 
+// Room for a staged output tile, where `least` bytes are left beside it.
+void plan_stage(TcParams& p, int out, int64_t least, int64_t& budget) {
+  const uint32_t bytes = ceil_div(2 * kTile * out, 1024) * 1024;
+  p.stage_bytes = out % 8 != 0 && least + bytes <= budget ? bytes : 0;
+  budget -= p.stage_bytes;
+}
+
 // Buffers for Y or dX. Shared memory goes first to the weights (as a
 // whole where two row tiles and two hidden buffers fit beside them), then to
 // whatever keeps the most work in flight.
@@ -715,7 +753,8 @@ void plan_rows(TcParams& p, bool bwd) {
   p.tmem_cols = pow2_cols(p.nb * g + p.ny * out);
   p.w_bytes = weight_bytes(p, p.nc);
   p.slices = static_cast<int>(std::min<int64_t>(p.tiles, sm_count()));
-  const int64_t budget = kSmemBudget;
+  int64_t budget = kSmemBudget;
+  plan_stage(p, bwd ? p.f.d : p.f.o, p.tile_bytes + p.h_bytes + 6 * kBlockBytes, budget);
   auto used = [&] { return static_cast<int64_t>(p.nx) * p.tile_bytes + p.nh * p.h_bytes; };
   p.nx = 2, p.nh = 2, p.slots = 1;
   p.resident = used() + p.w_bytes <= budget;
@@ -758,7 +797,8 @@ bool plan_weights(TcParams& p, bool dx) {
   p.slices = static_cast<int>(std::min<int64_t>(p.tiles, std::max(1, sm_count() / p.groups)));
   p.h_bytes = (p.split ? 2 : 3) * kBlockBytes;
   p.w_bytes = weight_bytes(p, p.cpc);
-  const int64_t budget = kSmemBudget;
+  int64_t budget = kSmemBudget;
+  if (dx) plan_stage(p, p.f.d, 2 * p.tile_bytes + p.h_bytes + p.w_bytes, budget);
   auto used = [&] { return static_cast<int64_t>(p.nx) * p.tile_bytes + p.nh * p.h_bytes; };
   const int tries[][2] = {{3, 2}, {2, 2}, {2, 1}, {1, 2}, {1, 1}};
   p.resident = 1, p.slots = p.slots_f = 0;
@@ -779,7 +819,7 @@ bool plan_weights(TcParams& p, bool dx) {
 
 uint32_t tc_smem(const TcParams& p) {
   return p.nx * p.tile_bytes + p.nh * p.h_bytes +
-         (p.resident ? p.w_bytes : p.slots * kBlockBytes) + 1024;
+         (p.resident ? p.w_bytes : p.slots * kBlockBytes) + p.stage_bytes + 1024;
 }
 
 int pack_weights(const TcParams& p, uint8_t* dst, cudaStream_t s) {
@@ -797,7 +837,7 @@ int launch_tc(TcParams p, cudaStream_t s) {
                                 smem));
   if (int rc = make_maps(p, kMode != kFwd)) return rc;
   const int out = kMode == kFwd ? p.f.o : p.f.d;
-  p.vec_y = out % 8 == 0 && aligned16(p.f.y);
+  p.vec_y = out % 8 == 0;
   ffn_tc_kernel<kMode><<<p.groups * p.slices, kTcThreads, smem, s>>>(p);
   TGS_LAUNCH_CHECK();
   return TGS_OK;
