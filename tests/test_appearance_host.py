@@ -85,6 +85,34 @@ def test_dropout_refusals():
         ap.dropout(x, 0.5, 0)
 
 
+def test_dropout_refuses_numbers_that_are_not_whole():
+    x = torch.zeros(5, 4)
+    with pytest.raises(TypeError):
+        ap.dropout(x, 0.5, 1.5)
+    with pytest.raises(TypeError):
+        ap.dropout(x, 0.5, 1, offset=2.5)
+
+
+def test_unaligned_bfloat16_rows_are_refused_below_python():
+    lib = _lib.load()
+    f = _lib.FfnArgs()
+    f.n, f.d, f.h, f.o, f.dtype = 4, 16, 8, 8, _lib.BF16
+    f.x = f.w_gate = f.w_up = f.w_down = f.y = f.scratch = 256
+    f.x_stride = 17
+    assert lib.tgs_ffn_fwd(ctypes.byref(f), None) == 1 and "aligned" in _lib.last_error()
+    f.x_stride, f.x = 16, 258
+    assert lib.tgs_ffn_fwd(ctypes.byref(f), None) == 1 and "aligned" in _lib.last_error()
+    f.x, f.y = 256, 260
+    assert lib.tgs_ffn_fwd(ctypes.byref(f), None) == 1 and "aligned" in _lib.last_error()
+    b = _lib.FfnBwdArgs()
+    f.y = 256
+    b.fwd, b.v_y, b.v_y_stride, b.v_x = f, 256, 12, 256
+    assert lib.tgs_ffn_bwd(ctypes.byref(b), None) == 1 and "aligned" in _lib.last_error()
+    assert lib.tgs_align_rows(None, 5, 0, 5, None, None) == 0
+    assert lib.tgs_align_rows(None, 5, 3, 5, None, None) == 1 and "NULL" in _lib.last_error()
+    assert lib.tgs_align_rows(256, 4, 3, 5, 256, None) == 1 and "overlap" in _lib.last_error()
+
+
 def test_appearance_colors_refusals():
     w = _ffn()
     with pytest.raises(ValueError, match="base"):

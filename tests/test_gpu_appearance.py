@@ -517,6 +517,65 @@ def test_two_streams_at_once():
                 assert torch.equal(a, e)
 
 
+@pytest.mark.parametrize("dtype,n,d,h,o", [(torch.float32, 9000, 128, 192, 64),
+                                           (torch.float32, 9000, 24, 48, 16),
+                                           (torch.bfloat16, 9000, 35, 100, 3),
+                                           (torch.bfloat16, 9000, 160, 320, 192)])
+def test_gated_feed_forward_captured_and_on_two_streams(dtype, n, d, h, o):
+    """Each of the block's kernels: a training step enqueued on two streams at
+    once, and one captured and replayed on other inputs."""
+    from tidegs_b200 import appearance as ap
+
+    def job(seed):
+        *ins, v = _ffn_inputs(n, d, h, o, dtype, seed)
+        return [t.requires_grad_(True) for t in ins], v
+
+    def train(leaves, v):
+        y = ap.gated_feed_forward(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, v))
+
+    jobs = [job(1), job(2)]
+    want = [train(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(3):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(train(*jobs[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for g in got[k]:
+            for a, e in zip(g, want[k]):
+                assert torch.equal(a, e)
+    leaves, v = jobs[0]
+    del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = train(leaves, v)
+    with torch.no_grad():
+        for t, other in zip(leaves, jobs[1][0]):
+            t.copy_(other)
+        v.copy_(jobs[1][1])
+    graph.replay()
+    for a, e in zip(held, want[1]):
+        assert torch.equal(a, e)
+    ap.check()
+
+
+@pytest.mark.parametrize("n,c", [(1, 1), (3, 7), (1000, 3), (129, 35), (70, 64), (33, 255)])
+def test_align_rows(n, c):
+    from tidegs_b200 import _lib
+
+    wide = _rand(_gen(3), n, c + 5, dtype=torch.bfloat16)
+    for src in (wide[:, :c].contiguous(), wide[:, 1:c + 1]):
+        units = -(-c // 8) * 8
+        out = torch.full((n, units), 7.0, dtype=torch.bfloat16, device="cuda")
+        _lib.call("tgs_align_rows", src.data_ptr(), src.stride(0) if n > 1 else c, n, c, out.data_ptr(),
+                  torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out[:, :c], src) and not out[:, c:].any()
+
+
 def test_other_device():
     from tidegs_b200 import appearance as ap
 

@@ -21,6 +21,7 @@ Kernels: tgs_layer_norm_fwd/bwd, tgs_ffn_fwd/bwd, tgs_dropout
 from __future__ import annotations
 
 import contextlib
+import operator
 from typing import Dict, Optional, Tuple, Union
 
 import torch
@@ -268,12 +269,15 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
                        w_down: torch.Tensor) -> torch.Tensor:
     """(silu(x w_gate^T) * (x w_up^T)) w_down^T for rows x [..., D]; w_gate
     and w_up [H, D], w_down [O, H]; D and O up to 256, H up to 4096; every
-    tensor float32 or every tensor bfloat16. Differentiable in all four. The
-    hidden values never reach memory: the backward computes them again.
+    tensor float32 or every tensor bfloat16. Differentiable in all four; the
+    hidden values are not kept: the backward computes them again. `check` tells
+    whether a kernel gave up waiting.
 
     bfloat16: the hidden values, and their gradients, are rounded to bfloat16
     between the products. float16 is refused: the hidden products leave its
-    range long before their inputs do."""
+    range long before their inputs do. float32: products of 32 bits; blocks of
+    12,288 multiply-adds a row and more keep a batch's hidden values in scratch
+    memory, take an infinity for NaN, and lose bits of values below 2^-100."""
     who = "gated_feed_forward"
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.dim() != 2 \
             or w_down.shape[1] != w_gate.shape[0]:
@@ -360,12 +364,13 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
         raise ValueError(f"{who}: x is {x.dtype}; float32, bfloat16 and float16 are supported")
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{who}: p {p} is not in [0, 1]")
+    seed = operator.index(seed)
     if not 0 <= seed < 2 ** 64:
         raise ValueError(f"{who}: seed {seed} is not a 64-bit unsigned number")
     if isinstance(offset, torch.Tensor):
         if offset.dtype != torch.int64 or offset.numel() != 1:
             raise ValueError(f"{who}: an offset tensor holds one int64")
-    elif not 0 <= offset < 2 ** 32:
+    elif not 0 <= operator.index(offset) < 2 ** 32:
         raise ValueError(f"{who}: offset {offset} is not a 32-bit unsigned number")
     if ids is not None and (ids.dtype != torch.int64 or tuple(ids.shape) != (n,)):
         raise ValueError(f"{who}: ids {ids.dtype} {tuple(ids.shape)} are not int64 [{n}]")
@@ -373,11 +378,11 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
     if isinstance(offset, torch.Tensor):
         _check(offset, who, "offset", x.device)
     else:
-        offset = int(offset)
+        offset = operator.index(offset)
     if ids is not None:
         _check(ids, who, "ids", x.device)
         ids = ids.contiguous()
-    args = (float(p), int(seed), offset, ids, bool(per_row))
+    args = (float(p), seed, offset, ids, bool(per_row))
     if _wants_grad(x):
         return _Dropout.apply(x, *args)
     return _dropout_run(x, *args)
