@@ -17,6 +17,11 @@
 // The same block of weights serves both products: as K-major operand of one
 // and as MN-major operand of the other.
 //
+// Rounding the hidden values to bf16 adds as much error to Y and dX as rounding
+// those does, 0.0024 of the result in place of 0.0017. A call of at most one
+// tile per SM, whose time is that of its launches, keeps them in two bf16 parts
+// (kFine) instead: 0.0017, and as long.
+//
 // Weights stay in shared memory where they fit (then the blocks lay them out
 // themselves); else a small kernel lays them out once per call and they
 // stream through a ring of 16 KB slots, out of L2.
@@ -49,7 +54,7 @@ struct TcParams {
   int kd, ko;      // 16-steps of D and O
   int nx, nh, nb, ny, slots, slots_f;  // buffers: row tiles, hidden, first and output accumulators
   int ycols;                  // columns of one output accumulator
-  int resident, vec_y;
+  int resident, vec_y, fine;
   uint32_t tile_bytes, h_bytes, w_bytes, stage_bytes;
   uint32_t tmem_cols;
   // Block b takes chunks [cpc g, cpc g + cpc) of tiles s, s + slices, ... with
@@ -193,30 +198,40 @@ __device__ __forceinline__ F2 one_plus_exp(F2 g) {
   return F2(fast_exp2(ea), fast_exp2(eb)) + F2(1.f, 1.f);
 }
 
+// Two values rounded and packed; with kFine also what the rounding left, in a
+// second bf16 part.
+template <bool kFine>
+__device__ __forceinline__ void round_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16(a, b);
+  if constexpr (kFine)
+    lo = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+
 // silu(g) u = g u / (1 + exp(-g)) of kW values, rounded and packed in pairs.
 // The special-function unit (16 results a cycle and SM) takes two operations a
 // value. One reciprocal for two values, 1 / a = b / (a b), saves a quarter of
 // them but costs as much again in products and moves: 196 against 168 us for
 // 2,097,152 rows of 64 -> 128 -> 48, and 168 with it for every second pair.
-template <int kW>
+template <bool kFine, int kW>
 __device__ __forceinline__ void gate(const float (&g)[kW], const float (&u)[kW],
-                                     uint32_t (&h)[kW / 2]) {
+                                     uint32_t (&h)[kW / 2], uint32_t (&lo)[kW / 2]) {
 #pragma unroll
   for (int i = 0; i < kW; i += 2) {
     const F2 g2(g[i], g[i + 1]);
     float a, b;
     one_plus_exp(g2).get(a, b);
     (g2 * F2(u[i], u[i + 1]) * F2(fast_rcp(a), fast_rcp(b))).get(a, b);
-    h[i / 2] = pack_bf16(a, b);
+    round_pair<kFine>(a, b, h[i / 2], lo[i / 2]);
   }
 }
 
 // The backward's hidden values, rounded and packed in pairs: dG, dU, and (for
 // the weights' gradients) h.
-template <bool kH, int kW>
+template <bool kH, bool kFine, int kW>
 __device__ __forceinline__ void gate_backward(const float (&g)[kW], const float (&u)[kW],
                                               const float (&dh)[kW], uint32_t (&h)[kW / 2],
-                                              uint32_t (&dg)[kW / 2], uint32_t (&du)[kW / 2]) {
+                                              uint32_t (&dg)[kW / 2], uint32_t (&du)[kW / 2],
+                                              uint32_t (&dg_lo)[kW / 2], uint32_t (&du_lo)[kW / 2]) {
 #pragma unroll
   for (int i = 0; i < kW; i += 2) {
     const F2 g2(g[i], g[i + 1]), u2(u[i], u[i + 1]), d2(dh[i], dh[i + 1]);
@@ -230,9 +245,9 @@ __device__ __forceinline__ void gate_backward(const float (&g)[kW], const float 
       h[i / 2] = pack_bf16(a, b);
     }
     (d2 * u2 * slope).get(a, b);
-    dg[i / 2] = pack_bf16(a, b);
+    round_pair<kFine>(a, b, dg[i / 2], dg_lo[i / 2]);
     (d2 * act).get(a, b);
-    du[i / 2] = pack_bf16(a, b);
+    round_pair<kFine>(a, b, du[i / 2], du_lo[i / 2]);
   }
 }
 
@@ -325,7 +340,7 @@ __host__ __device__ __forceinline__ int chunk_floats(const TcParams& p) {
 }
 
 // --- the kernel --------------------------------------------------------------------
-template <int kMode>
+template <int kMode, bool kFine>
 __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_constant__ TcParams p) {
   extern __shared__ uint8_t raw[];
   __shared__ TcBars bars;
@@ -337,6 +352,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
   // from lane 0, so that the compiler sees the roles' branches as uniform
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr bool kBwd = kMode != kFwd, kHasDw = kMode >= kDw, kRows = kMode != kDw;
+  constexpr uint32_t kLoAt = (kBwd ? 2 : 1) * kBlockBytes;  // second parts in a hidden buffer
   const int group_id = kHasDw ? blockIdx.x % p.groups : 0;
   const int slice = kHasDw ? blockIdx.x / p.groups : blockIdx.x;
   const bool want_gu = !kHasDw || !p.split || !(group_id & 1);  // dWg and dWu
@@ -405,7 +421,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
       // whole 16-steps of the chunk's hidden values
       const int cols = (min(kChunk, p.f.h - (j0 + j) * kChunk) + 15) & ~15;
       constexpr int kParts = kBwd ? 3 : 2;  // G, U, dH
-      constexpr int kW = kHasDw ? 8 : 16;   // what the registers hold
+      constexpr int kW = kHasDw || kFine ? 8 : 16;  // what the registers hold
       constexpr int kTurns = kChunk / kW / 2;
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
@@ -431,16 +447,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
           warp_arrive(&bars.gempty[group], lane);  // the accumulators have been read
         }
         if (q * kW < cols) {
-          uint32_t h[kW / 2], dg[kW / 2], du[kW / 2];
+          uint32_t h[kW / 2], dg[kW / 2], du[kW / 2], lo[kW / 2], lo2[kW / 2];
           if constexpr (kBwd) {
-            gate_backward<kHasDw>(v[0], v[1], v[kParts - 1], h, dg, du);
+            gate_backward<kHasDw, kFine>(v[0], v[1], v[kParts - 1], h, dg, du, lo, lo2);
           } else {
-            gate(v[0], v[1], h);
+            gate<kFine>(v[0], v[1], h, lo);
           }
           if (kMode == kFwd || (kHasDw && want_d)) store_granule(hbuf, row, q, h);
           if (kBwd && want_gu) {
             store_granule(hbuf + dg_at, row, q, dg);
             store_granule(hbuf + dg_at + kBlockBytes, row, q, du);
+          }
+          if constexpr (kFine) {
+            store_granule(hbuf + kLoAt, row, q, lo);
+            if constexpr (kBwd) store_granule(hbuf + kLoAt + kBlockBytes, row, q, lo2);
           }
         }
       }
@@ -526,6 +546,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
                             id, ks, j > 0);
             tc_mma_steps<4>(y + 64 * c, desc_k(h + dg_at + kBlockBytes), kStepK,
                             desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
+            if constexpr (kFine) {
+              tc_mma_steps<4>(y + 64 * c, desc_k(h + kLoAt), kStepK, desc_mn(w, kBlockBytes),
+                              kStepMn, id, ks, true);
+              tc_mma_steps<4>(y + 64 * c, desc_k(h + kLoAt + kBlockBytes), kStepK,
+                              desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
+            }
             release();
           }
         }
@@ -536,6 +562,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
             tc_mma_steps<4>(y + 128 * b8, desc_k(h), kStepK, desc_k(w), kStepK,
                             tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
                             j > 0);
+            if constexpr (kFine)
+              tc_mma_steps<4>(y + 128 * b8, desc_k(h + kLoAt), kStepK, desc_k(w), kStepK,
+                              tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
+                              true);
             release();
           }
         }
@@ -724,6 +754,7 @@ TcParams tc_params(const FfnParams& f) {
   p.cd = ceil_div(f.d, 64), p.co = ceil_div(f.o, 64), p.nc = ceil_div(f.h, kChunk);
   p.tiles = ceil_div<int64_t>(f.n, kTile);
   p.cpc = p.nc, p.groups = 1;
+  p.fine = p.tiles <= sm_count();
   return p;
 }
 
@@ -745,7 +776,7 @@ void plan_stage(TcParams& p, int out, int64_t least, int64_t& budget) {
 // whatever keeps the most work in flight.
 void plan_rows(TcParams& p, bool bwd) {
   p.tile_bytes = (p.cd + (bwd ? p.co : 0)) * kBlockBytes;
-  p.h_bytes = (bwd ? 2 : 1) * kBlockBytes;
+  p.h_bytes = (bwd ? 2 : 1) * (p.fine ? 2 : 1) * kBlockBytes;
   const uint32_t out = bwd ? p.kd * 16 : p.ko * 16, g = bwd ? 192 : 128;
   p.nb = 2 * g + out <= 512 ? 2 : 1;
   p.ny = p.nb * g + 2 * out <= 512 ? 2 : 1;
@@ -828,17 +859,17 @@ int pack_weights(const TcParams& p, uint8_t* dst, cudaStream_t s) {
   return TGS_OK;
 }
 
-template <int kMode>
+template <int kMode, bool kFine = false>
 int launch_tc(TcParams p, cudaStream_t s) {
   const int smem = static_cast<int>(tc_smem(p));
   // Before the tensor maps: this binds the thread's context, which a thread of
   // autograd's may not have yet and the encoder needs.
-  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                smem));
+  TGS_CUDA(cudaFuncSetAttribute(ffn_tc_kernel<kMode, kFine>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (int rc = make_maps(p, kMode != kFwd)) return rc;
   const int out = kMode == kFwd ? p.f.o : p.f.d;
   p.vec_y = out % 8 == 0;
-  ffn_tc_kernel<kMode><<<p.groups * p.slices, kTcThreads, smem, s>>>(p);
+  ffn_tc_kernel<kMode, kFine><<<p.groups * p.slices, kTcThreads, smem, s>>>(p);
   TGS_LAUNCH_CHECK();
   return TGS_OK;
 }
@@ -854,7 +885,7 @@ struct BwdPlan {
 BwdPlan plan_backward(const FfnParams& f, bool dx, bool dw) {
   BwdPlan b{};
   b.rows = b.weights = tc_params(f);
-  b.both = dx && dw && plan_weights(b.weights, true);
+  b.both = dx && dw && !b.weights.fine && plan_weights(b.weights, true);
   bool packed = false;
   if (dw && !b.both) {
     b.weights = tc_params(f);
@@ -904,7 +935,7 @@ int ffn_tc_forward(const FfnParams& f, cudaStream_t s) {
     p.packed = reinterpret_cast<const uint8_t*>(f.scratch);
     if (int rc = pack_weights(p, reinterpret_cast<uint8_t*>(f.scratch), s)) return rc;
   }
-  return launch_tc<kFwd>(p, s);
+  return p.fine ? launch_tc<kFwd, true>(p, s) : launch_tc<kFwd>(p, s);
 }
 
 int64_t ffn_tc_scratch_floats(int64_t n, int d, int h, int o, bool backward) {
@@ -930,7 +961,7 @@ int ffn_tc_backward(const FfnParams& f, cudaStream_t s) {
   }
   b.weights.partial = f.scratch;
   if (dx && !b.both) {
-    if (int rc = launch_tc<kDx>(b.rows, s)) return rc;
+    if (int rc = b.rows.fine ? launch_tc<kDx, true>(b.rows, s) : launch_tc<kDx>(b.rows, s)) return rc;
   }
   if (!dw) return TGS_OK;
   if (int rc = b.both ? launch_tc<kDxDw>(b.weights, s) : launch_tc<kDw>(b.weights, s)) return rc;
