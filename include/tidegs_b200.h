@@ -860,10 +860,10 @@ typedef struct {
 
 /* y = (silu(x w_gate^T) * (x w_up^T)) w_down^T. bf16: one kernel (a second one
  * lays out weights that do not fit shared memory), hidden values rounded to
- * bf16; fp32: one kernel, or from 12,288 multiply-adds a row on products on the
- * tensor cores with a batch's hidden values in scratch. The error word tells of
- * a wait that ran out (TGS_DEV_WAIT_TIMEOUT); the kernels run whatever it
- * holds. */
+ * bf16 (to two bf16 parts in calls of at most 128 rows per SM). fp32: one
+ * kernel, or, from 12,288 multiply-adds a row on, products on the tensor cores
+ * with a batch's hidden values in scratch. The error word tells of a wait that
+ * ran out (TGS_DEV_WAIT_TIMEOUT); the kernels run whatever it holds. */
 TGS_API int tgs_ffn_fwd(const TgsFfnArgs* args, void* stream);
 
 /* Floats of scratch that tgs_ffn_fwd (backward = 0) or tgs_ffn_bwd (1) needs

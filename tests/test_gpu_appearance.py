@@ -217,9 +217,12 @@ def _ffn_inputs(n, d, h, o, dtype, seed=0):
             _rand(g, n, o, dtype=dtype, scale=0.1))
 
 
-def _ffn_expect(x, wg, wu, wd, v, dtype):
+def _ffn_expect(x, wg, wu, wd, v, dtype, parts=1):
+    """`parts`: bf16 parts of a hidden value; the last leaves half its step, 2^-8
+    of what the others left."""
     x, wg, wu, wd, v = (V(t) for t in (x, wg, wu, wd, v))
-    hid = (lambda t: t.stored(dtype)) if dtype == torch.bfloat16 else (lambda t: t)
+    hid = (lambda t: V(t.val, t.err + HALF[dtype] ** parts * t.most + TINY[dtype])) \
+        if dtype == torch.bfloat16 else (lambda t: t)
     g, u = x @ wg.T, x @ wu.T
     # exp and the quotient: a few steps, and one per unit of the exponent
     wave = (16 + 2 * g.most) * U
@@ -331,6 +334,21 @@ def test_gated_feed_forward_partial_gradients_agree():
         for k in range(4):
             part = [t.detach().requires_grad_(i == k) for i, t in enumerate(leaves)]
             assert torch.equal(torch.autograd.grad(ap.gated_feed_forward(*part), part[k], v)[0], full[k])
+
+
+@pytest.mark.parametrize("n,d,h,o", [(1, 35, 96, 3), (40, 10, 24, 88), (500, 145, 72, 9),
+                                     (1500, 32, 64, 3), (700, 192, 300, 128), (300, 256, 500, 256)])
+def test_small_bfloat16_calls_round_once(n, d, h, o):
+    """A call of one tile per SM keeps hidden values in two bf16 parts."""
+    from tidegs_b200 import appearance as ap
+
+    *ins, v = _ffn_inputs(n, d, h, o, torch.bfloat16, 3)
+    leaves = [t.requires_grad_(True) for t in ins]
+    y = ap.gated_feed_forward(*leaves)
+    grads = torch.autograd.grad(y, leaves, v)
+    want = _ffn_expect(*(t.detach() for t in ins), v, torch.bfloat16, parts=2)
+    for (name, e), got in zip(want.items(), (y, *grads)):
+        _far(got, e, name)
 
 
 def test_gated_feed_forward_gradient_matches_differences():
@@ -574,6 +592,22 @@ def test_align_rows(n, c):
         _lib.call("tgs_align_rows", src.data_ptr(), src.stride(0) if n > 1 else c, n, c, out.data_ptr(),
                   torch.cuda.current_stream().cuda_stream)
         assert torch.equal(out[:, :c], src) and not out[:, c:].any()
+
+
+def test_check_reads_the_error_word():
+    """A wait that ran out is told by check() (the word is set by hand)."""
+    from tidegs_b200 import appearance as ap
+
+    *ins, _ = _ffn_inputs(10, 16, 16, 16, torch.bfloat16)
+    ap.gated_feed_forward(*ins)
+    ap.check()
+    ap.check("cuda")
+    word = ap._err_words[ins[0].device]
+    word[0] = 4
+    with pytest.raises(RuntimeError, match="timed out"):
+        ap.check("cuda")
+    word.zero_()
+    ap.check(ins[0].device)
 
 
 def test_other_device():

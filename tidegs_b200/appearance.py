@@ -185,7 +185,9 @@ def check(device=None) -> None:
     """Raises if a bounded wait inside an earlier gated_feed_forward kernel on
     `device` (default: the current one) ran out, which leaves that call's
     results undefined. Waits for the device."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     word = _err_words.get(device)
     if word is None:
         return
@@ -274,7 +276,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     whether a kernel gave up waiting.
 
     bfloat16: the hidden values, and their gradients, are rounded to bfloat16
-    between the products. float16 is refused: the hidden products leave its
+    between the products (calls of at most 128 rows per SM: to two bfloat16
+    parts, 16 bits). float16 is refused: the hidden products leave its
     range long before their inputs do. float32: products of 32 bits; blocks of
     12,288 multiply-adds a row and more keep a batch's hidden values in scratch
     memory, take an infinity for NaN, and lose bits of values below 2^-100."""

