@@ -158,8 +158,16 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(const NormParams
   }
 }
 
+// Blocks to an SM that the compiler has to leave registers for (0: it chooses).
+// Rows of many values to a thread are held back by too few of them: 100,003
+// rows of 768 bf16 (24 values) 138 us with two, 185 with the one that it chose;
+// 300,000 of 301 fp32 (16) 522 against 698; the others lose by it.
+constexpr int norm_min_blocks(int values, bool block) {
+  return block || values < 16 ? 0 : values <= 24 ? 2 : 1;
+}
+
 template <class T, int kVec, int kNv, int kU, bool kBlock>
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, norm_min_blocks(kVec * kNv, kBlock)) norm_bwd_kernel(const NormParams p) {
   extern __shared__ float acc[];  // [2, C]: the block's parameter gradients
   __shared__ float red[kNormThreads / 32][kU];
   const int lanes = p.lanes, c = p.c;
