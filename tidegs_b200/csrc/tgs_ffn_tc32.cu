@@ -339,7 +339,10 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
           for (int i = 0; i < 64; ++i)
             if (c0 + i < width) sum[i >> 4][i & 15] += to[c0 + i];
         }
-        const bool vec = width % 4 == 0 && aligned16(p.out);
+        // The output's rows start on 16-byte boundaries where their width allows it;
+        // rows of the weights' gradients only if what lies before them in the
+        // slices is whole vectors too.
+        const bool vec = width % 4 == 0 && aligned16(to);
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {
           const float* v = &sum[i >> 4][i & 15];
