@@ -322,8 +322,11 @@ int launch_norm(NormParams p, cudaStream_t s, int* blocks) {
   p.lanes = kBlock ? kNormThreads : norm_lanes(p.c, kVec * kNv);
   const int64_t rows = static_cast<int64_t>(kNormThreads / p.lanes) * kU;
   const int smem = kBwd && p.partial ? 2 * p.c * static_cast<int>(sizeof(float)) : 0;
-  if (smem > 48 * 1024)
-    TGS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // The default limit, 48 KB, covers the kernel's own arrays too. One limit for
+  // every width: it belongs to the kernel, and another thread may be launching it.
+  constexpr int kMostSmem = 2 * kNormMaxC * static_cast<int>(sizeof(float));
+  if (smem > 32 * 1024)
+    TGS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
   // As many blocks as are resident at once: each sums its parameter gradients
   // and hands them over once.
   static int resident = 0;
