@@ -47,3 +47,49 @@ for dtype in TYPES:
     for c in (6136, 6140, 6141, 6143, 6144, 6145, 6152):
         _norm_check(*_norm_inputs(3, c, dtype, dtype))
 """)
+
+
+# --- derivatives that are not offered ------------------------------------------------
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent is not dropped."""
+    from torch.autograd import forward_ad
+
+    from tidegs_b200 import appearance as ap
+
+    x, wg, wu, wd, _ = _ffn_inputs(20, 16, 24, 8, torch.float32)
+    w, b = torch.ones(16, device="cuda"), torch.zeros(16, device="cuda")
+    calls = [(lambda *a: ap.layer_norm(*a), [x, w, b]), (lambda *a: ap.gated_feed_forward(*a), [x, wg, wu, wd]),
+             (lambda a: ap.dropout(a, 0.5, 1), [x])]
+    with forward_ad.dual_level():
+        for f, args in calls:
+            f(*args)  # no tangent: as ever
+            for k in range(len(args)):
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == k else t for i, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    f(*dual)
+                with forward_ad._set_fwd_grad_enabled(False):
+                    f(*dual)
+            leaf = args[0].detach().requires_grad_(True)
+            y = f(leaf, *args[1:])
+            v = torch.ones_like(y)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, forward_ad.make_dual(v, v.clone()), retain_graph=True)
+            torch.autograd.grad(y, leaf, v)
+
+
+@pytest.mark.parametrize("transform", ["grad", "jvp", "vmap"])
+def test_function_transforms_are_refused(transform):
+    from tidegs_b200 import appearance as ap
+
+    x, wg, wu, wd, _ = _ffn_inputs(20, 16, 24, 8, torch.float32)
+    for f in (ap.layer_norm, lambda a: ap.gated_feed_forward(a, wg, wu, wd), lambda a: ap.dropout(a, 0.5, 1)):
+        with pytest.raises(RuntimeError):
+            if transform == "grad":
+                torch.func.grad(lambda a: f(a).sum())(x)
+            elif transform == "jvp":
+                torch.func.jvp(f, (x,), (torch.ones_like(x),))
+            else:
+                torch.func.vmap(f)(x[:, None])

@@ -9,11 +9,11 @@ in exposure, weather or time of day. No counterpart in the reference.
                          a mask that is drawn again instead of stored
     appearance_colors    the three of them added to SH colors or coefficients
 
-All are differentiable (first order) and run on the current stream of the
-tensors' device. Inputs are CUDA tensors [..., C]; columns of any stride are
-taken (those whose rows are not contiguous values are copied first). Sums are
-in 32 bits, outputs are rounded once to their type. Every kernel adds in a
-fixed order: the same call gives the same bits.
+All are differentiable (first order, reverse mode; others are refused) and run
+on the current stream of the tensors' device. Inputs are CUDA tensors [..., C];
+columns of any stride are taken (those whose rows are not contiguous values are
+copied first). Sums are in 32 bits, outputs are rounded once to their type.
+Every kernel adds in a fixed order: the same call gives the same bits.
 
 Kernels: tgs_layer_norm_fwd/bwd, tgs_ffn_fwd/bwd, tgs_dropout
 (libtidegs_b200.so).
@@ -25,6 +25,7 @@ import operator
 from typing import Dict, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -72,7 +73,14 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _wants_grad(*ts: Optional[torch.Tensor]) -> bool:
+def _refuse_tangents(who: str, *ts: Optional[torch.Tensor]) -> None:
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{who}: forward-mode derivatives are not supported")
+
+
+def _wants_grad(who: str, *ts: Optional[torch.Tensor]) -> bool:
+    _refuse_tangents(who, *ts)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
@@ -113,6 +121,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, v_y):
+        _refuse_tangents("layer_norm", v_y)
         x, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         c = x.shape[-1]
@@ -163,7 +172,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is not None:
             _check(t, who, name, x.device)
-    if _wants_grad(x, weight, bias):
+    if _wants_grad(who, x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _norm_forward(x, weight, bias, float(eps))
 
@@ -251,6 +260,7 @@ class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, v_y):
+        _refuse_tangents("gated_feed_forward", v_y)
         x, *weights = ctx.saved_tensors
         weights = [w.contiguous() for w in weights]
         need_x, *need_w = ctx.needs_input_grad
@@ -300,7 +310,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         if w.dtype != x.dtype:
             raise ValueError(f"{who}: {name} is {w.dtype}, x {x.dtype}")
         _check(w, who, name, x.device)
-    if _wants_grad(x, w_gate, w_up, w_down):
+    if _wants_grad(who, x, w_gate, w_up, w_down):
         return _GatedFeedForward.apply(x, w_gate, w_up, w_down)
     return _ffn_forward(x, w_gate, w_up, w_down)
 
@@ -336,6 +346,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, v_y):
+        _refuse_tangents("dropout", v_y)
         ids, offset_dev = ctx.saved_tensors
         p, seed, offset, per_row = ctx.args
         offset = offset_dev if offset is None else offset
@@ -386,7 +397,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: Union[int, torch.Tenso
         _check(ids, who, "ids", x.device)
         ids = ids.contiguous()
     args = (float(p), seed, offset, ids, bool(per_row))
-    if _wants_grad(x):
+    if _wants_grad(who, x):
         return _Dropout.apply(x, *args)
     return _dropout_run(x, *args)
 
