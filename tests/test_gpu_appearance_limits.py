@@ -93,3 +93,26 @@ def test_function_transforms_are_refused(transform):
                 torch.func.jvp(f, (x,), (torch.ones_like(x),))
             else:
                 torch.func.vmap(f)(x[:, None])
+
+
+# --- values near the ends of their range ----------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [4, 20000])
+@pytest.mark.parametrize("d,h,o", [(2, 3, 2), (64, 128, 48), (160, 320, 192)])
+def test_closed_gates_of_large_values(dtype, n, d, h, o):
+    """silu(-1e25) is -0, so the block is 0 times what passes the gate, however
+    large that is; the same for the gate's slope and the gradients."""
+    from tidegs_b200 import appearance as ap
+
+    x = torch.zeros(n, d, device="cuda", dtype=dtype)
+    x[:, 0], x[:, 1] = -1e25, 1e25
+    wg, wu = torch.zeros(2, h, d, device="cuda", dtype=dtype)
+    wg[:, 0] = wu[:, 1] = 1.0
+    wd = torch.ones(o, h, device="cuda", dtype=dtype)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = ap.gated_feed_forward(*leaves)
+    assert not y.any() and not torch.isnan(y).any()
+    v = torch.full((n, o), 1e20, device="cuda", dtype=dtype)
+    for name, t in zip(("v_x", "v_w_gate", "v_w_up", "v_w_down"), torch.autograd.grad(y, leaves, v)):
+        assert not torch.isnan(t).any() and not t.any(), name

@@ -160,7 +160,7 @@ struct Tile {
           dh[j][i].get(da, db);
           float* next = to + (kH ? kHid * kLd : 0);
           *reinterpret_cast<float2*>(next + 2 * i) =
-              make_float2(da * ua * (sa + aa * (1.f - sa)), db * ub * (sb + ab * (1.f - sb)));
+              make_float2((sa + aa * (1.f - sa)) * ua * da, (sb + ab * (1.f - sb)) * ub * db);
           *reinterpret_cast<float2*>(next + kHid * kLd + 2 * i) = make_float2(da * aa, db * ab);
         }
       }

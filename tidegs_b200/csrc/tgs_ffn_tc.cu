@@ -212,7 +212,8 @@ __device__ __forceinline__ void round_pair(float a, float b, uint32_t& hi, uint3
     lo = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
 }
 
-// silu(g) u = g u / (1 + exp(-g)) of kW values, rounded and packed in pairs.
+// silu(g) u = g / (1 + exp(-g)) u of kW values, rounded and packed in pairs. The
+// gate comes first: a closed one gives 0 however large g u is.
 // The special-function unit (16 results a cycle and SM) takes two operations a
 // value. One reciprocal for two values, 1 / a = b / (a b), saves a quarter of
 // them but costs as much again in products and moves: 196 against 168 us for
@@ -225,7 +226,7 @@ __device__ __forceinline__ void gate(const float (&g)[kW], const float (&u)[kW],
     const F2 g2(g[i], g[i + 1]);
     float a, b;
     one_plus_exp(g2).get(a, b);
-    (g2 * F2(u[i], u[i + 1]) * F2(fast_rcp(a), fast_rcp(b))).get(a, b);
+    (g2 * F2(fast_rcp(a), fast_rcp(b)) * F2(u[i], u[i + 1])).get(a, b);
     round_pair<kFine>(a, b, h[i / 2], lo[i / 2]);
   }
 }
@@ -250,7 +251,7 @@ __device__ __forceinline__ void gate_backward(const float (&g)[kW], const float 
       (act * u2).get(a, b);
       round_pair<kFine>(a, b, h[i / 2], h_lo[i / 2]);
     }
-    (d2 * u2 * slope).get(a, b);
+    (slope * u2 * d2).get(a, b);
     round_pair<kFine>(a, b, dg[i / 2], dg_lo[i / 2]);
     (d2 * act).get(a, b);
     round_pair<kFine>(a, b, du[i / 2], du_lo[i / 2]);

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads32) ffn_tc32_kernel(const __grid_const
             h[i] = act * u;
             if constexpr (kJob == kHiddenBwd) {
               const float d = sum[4 + q][8 * u8 + i];
-              dg[i] = d * u * (sg + act * (1.f - sg));
+              dg[i] = (sg + act * (1.f - sg)) * u * d;
               du[i] = d * act;
             }
           }
