@@ -3,8 +3,10 @@ documentation allows: layouts whose parts start off 16-byte boundaries, widths
 at a limit, several host threads, derivatives that are not offered, values near
 the ends of their range, sums over very many rows. Tolerances are those of
 test_gpu_appearance.py unless a test derives its own."""
+import ctypes
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
@@ -116,3 +118,42 @@ def test_closed_gates_of_large_values(dtype, n, d, h, o):
     v = torch.full((n, o), 1e20, device="cuda", dtype=dtype)
     for name, t in zip(("v_x", "v_w_gate", "v_w_up", "v_w_down"), torch.autograd.grad(y, leaves, v)):
         assert not torch.isnan(t).any() and not t.any(), name
+
+
+# --- several host threads -----------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,sizes", [(torch.float32, [(60, 35, 96, 3), (60, 8, 40, 3)]),
+                                         (torch.float32, [(60, 35, 96, 40), (60, 8, 40, 40)]),
+                                         (torch.bfloat16, [(60, 256, 512, 256), (60, 16, 16, 16)])])
+def test_one_kernel_at_two_sizes_of_shared_memory_from_two_threads(dtype, sizes):
+    """Launches of one kernel that want different shared memory, from two host
+    threads at once: none is refused, each gives what it gives alone."""
+    from tidegs_b200 import _lib
+    from tidegs_b200 import appearance as ap
+
+    lib, jobs = _lib.load(), []
+    for k, size in enumerate(sizes):
+        *ins, _ = _ffn_inputs(*size, dtype, k)
+        args, scratch = ap._ffn_args(*ins, backward=False)
+        y = torch.empty(size[0], size[3], dtype=dtype, device="cuda")
+        args.y = y.data_ptr()
+        jobs.append((args, torch.cuda.Stream(), y, ap.gated_feed_forward(*ins), ins, scratch))
+    torch.cuda.synchronize()
+    start, problems = threading.Barrier(len(jobs)), []
+
+    def run(args, stream):
+        start.wait(30)
+        for _ in range(20000):
+            if lib.tgs_ffn_fwd(ctypes.byref(args), stream.cuda_stream):
+                problems.append(_lib.last_error())
+                return
+
+    threads = [threading.Thread(target=run, args=job[:2]) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    torch.cuda.synchronize()
+    assert not problems, problems
+    for _, _, y, want, *_ in jobs:
+        assert torch.equal(y, want)

@@ -384,6 +384,8 @@ int tile_smem(const FfnParams& p, int r, bool bwd, int hidden, int tiles, int we
   return 4 * ((tiles * (p.d + (bwd ? p.o : 0)) + hidden * kHid) * rows_ld(r) +
               weights * (p.d * kLdW + p.o * kLdD));
 }
+// All that a block can have; the kernels' limit at every size, since it belongs
+// to the kernel and another thread may be launching it at another size.
 constexpr int kMostSmem = 227 * 1024;
 
 int ffn_slices(int64_t n, int d, int h, int o) {
@@ -401,7 +403,7 @@ int launch_rows(const FfnParams& p, cudaStream_t s) {
   int smem = tile_smem(p, kR, kBwd, kBwd ? 2 : 1, 1, 2), buffers = 2;
   if (p.h <= kHid || smem > kMostSmem) smem = tile_smem(p, kR, kBwd, kBwd ? 2 : 1, 1, 1), buffers = 1;
   TGS_CUDA(cudaFuncSetAttribute(ffn_rows_kernel<kR, kBwd, kCols>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
   ffn_rows_kernel<kR, kBwd, kCols>
       <<<static_cast<unsigned>(ceil_div<int64_t>(p.n, 16 * kR)), kThreads, smem, s>>>(p, buffers);
   TGS_LAUNCH_CHECK();
@@ -423,7 +425,7 @@ int launch_weights(const FfnParams& p, int slices, cudaStream_t s) {
   int smem = tile_smem(p, kR, true, 3, 2, 1), buffers = 2;
   if (smem > kMostSmem) smem = tile_smem(p, kR, true, 3, 1, 1), buffers = 1;
   TGS_CUDA(cudaFuncSetAttribute(ffn_weights_kernel<kR, kCols>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
   ffn_weights_kernel<kR, kCols><<<dim3(ceil_div(p.h, kHid), slices), kThreads, smem, s>>>(p, buffers);
   TGS_LAUNCH_CHECK();
   return TGS_OK;

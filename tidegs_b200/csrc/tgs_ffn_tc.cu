@@ -32,6 +32,8 @@
 // stream through a ring of 16 KB slots, out of L2.
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "tgs_ffn.cuh"
 #include "tgs_tc.cuh"
 
@@ -878,10 +880,11 @@ int pack_weights(const TcParams& p, uint8_t* dst, cudaStream_t s) {
 template <int kMode, bool kFine = false>
 int launch_tc(TcParams p, cudaStream_t s) {
   const int smem = static_cast<int>(tc_smem(p));
-  // Before the tensor maps: this binds the thread's context, which a thread of
-  // autograd's may not have yet and the encoder needs.
+  // One limit for calls of every size: it belongs to the kernel, and another
+  // thread may be launching it. Before the tensor maps: this binds the thread's
+  // context, which a thread of autograd's may not have yet and the encoder needs.
   TGS_CUDA(cudaFuncSetAttribute(ffn_tc_kernel<kMode, kFine>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget + 1024));
   if (int rc = make_maps(p, kMode != kFwd)) return rc;
   const int out = kMode == kFwd ? p.f.o : p.f.d;
   p.vec_y = out % 8 == 0;
@@ -921,13 +924,15 @@ BwdPlan plan_backward(const FfnParams& f, bool dx, bool dw) {
 }  // namespace
 
 int make_row_map(CUtensorMap* map, const void* base, int64_t rows, int cols, int64_t stride) {
-  static decltype(&cuTensorMapEncodeTiled) encode = nullptr;
+  static std::atomic<decltype(&cuTensorMapEncodeTiled)> known{nullptr};
+  auto encode = known.load(std::memory_order_relaxed);
   if (encode == nullptr) {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult found;
     TGS_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found));
     TGS_CHECK_ARG(fn != nullptr, "cuTensorMapEncodeTiled is missing from the driver");
     encode = reinterpret_cast<decltype(encode)>(fn);
+    known.store(encode, std::memory_order_relaxed);
   }
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};

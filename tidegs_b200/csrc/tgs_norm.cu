@@ -15,6 +15,8 @@
 // Measured: 2,097,152 rows of 64 bf16, forward 104 us (5.2 TB/s, 80 % of the
 // copy rate), backward 197 us; of 64 fp32 186 and 255 us (5.8 and 6.3 TB/s);
 // 786,432 rows of 59 fp32, which only take single loads, 83 and 157 us.
+#include <atomic>
+
 #include "tgs_common.cuh"
 #include "tgs_vec.cuh"
 
@@ -329,11 +331,13 @@ int launch_norm(NormParams p, cudaStream_t s, int* blocks) {
     TGS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
   // As many blocks as are resident at once: each sums its parameter gradients
   // and hands them over once.
-  static int resident = 0;
+  static std::atomic<int> known{0};
+  int resident = known.load(std::memory_order_relaxed);
   if (resident == 0) {
     int n = 0;
     TGS_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kNormThreads, 0));
     resident = std::max(1, std::min(n, kNormBlocksPerSm));
+    known.store(resident, std::memory_order_relaxed);
   }
   *blocks = static_cast<int>(std::min<int64_t>(ceil_div<int64_t>(p.n, rows),
                                                static_cast<int64_t>(sm_count()) * resident));
