@@ -157,3 +157,14 @@ def test_one_kernel_at_two_sizes_of_shared_memory_from_two_threads(dtype, sizes)
     assert not problems, problems
     for _, _, y, want, *_ in jobs:
         assert torch.equal(y, want)
+
+
+def test_the_rows_gradient_is_the_same_alone():
+    """With the weights' gradients, from one kernel, and without them."""
+    from tidegs_b200 import appearance as ap
+
+    x, wg, wu, wd, v = _ffn_inputs(20000, 64, 128, 48, torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    full = torch.autograd.grad(ap.gated_feed_forward(*leaves), leaves, v)[0]
+    alone = torch.autograd.grad(ap.gated_feed_forward(x, *(t.detach() for t in leaves[1:])), x, v)[0]
+    assert torch.equal(full, alone)

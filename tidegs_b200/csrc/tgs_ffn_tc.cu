@@ -246,16 +246,17 @@ __device__ __forceinline__ void gate_backward(const float (&g)[kW], const float 
     const F2 g2(g[i], g[i + 1]), u2(u[i], u[i + 1]), d2(dh[i], dh[i + 1]);
     float a, b;
     one_plus_exp(g2).get(a, b);
-    const F2 s2(fast_rcp(a), fast_rcp(b)), act = g2 * s2;
-    // silu'(g) = s + act (1 - s)
-    const F2 slope = fma2(act, fma2(s2, F2(-1.f, -1.f), F2(1.f, 1.f)), s2);
+    // s dh first: a closed gate gives 0 however large dh u is. silu'(g) =
+    // s (1 + g (1 - s)).
+    const F2 s2(fast_rcp(a), fast_rcp(b)), sd = s2 * d2;
+    const F2 slope = fma2(g2, fma2(s2, F2(-1.f, -1.f), F2(1.f, 1.f)), F2(1.f, 1.f));
     if constexpr (kH) {
-      (act * u2).get(a, b);
+      (g2 * s2 * u2).get(a, b);
       round_pair<kFine>(a, b, h[i / 2], h_lo[i / 2]);
     }
-    (slope * u2 * d2).get(a, b);
+    (sd * u2 * slope).get(a, b);
     round_pair<kFine>(a, b, dg[i / 2], dg_lo[i / 2]);
-    (d2 * act).get(a, b);
+    (g2 * sd).get(a, b);
     round_pair<kFine>(a, b, du[i / 2], du_lo[i / 2]);
   }
 }
