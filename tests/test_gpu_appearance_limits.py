@@ -12,7 +12,8 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_gpu_appearance import _ffn_check, _ffn_inputs
+from oracle import appearance as orc
+from test_gpu_appearance import HALF, _ffn_check, _ffn_inputs, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +169,58 @@ def test_the_rows_gradient_is_the_same_alone():
     full = torch.autograd.grad(ap.gated_feed_forward(*leaves), leaves, v)[0]
     alone = torch.autograd.grad(ap.gated_feed_forward(x, *(t.detach() for t in leaves[1:])), x, v)[0]
     assert torch.equal(full, alone)
+
+
+# --- sums over very many rows ---------------------------------------------------------
+
+def test_bfloat16_gradients_of_one_sign_over_many_rows():
+    """One slice of rows (4096 hidden values of the widest block leave no SM for
+    a second), all products of one sign, so that what additions cut off adds up:
+    the mean error of the gradient is what they lose: 8192 values of scattered
+    sizes, each rounded to bfloat16 either way by at most 2^-8, shift the mean by
+    less than 2^-8 / sqrt(8192) = 4.3e-5. A sum grows evenly over at most 1,024
+    instructions, each of which may cut off two units of 2^-23 of what the sum
+    is by then: 1,024 / 2 x 2 x 2^-23 = 1.2e-4."""
+    from tidegs_b200 import appearance as ap
+
+    n, d, h, o = 300_000, 256, 4096, 256
+    g = _gen(5)
+    x = torch.rand(n, d, generator=g, device="cuda").bfloat16()
+    wg, wu = ((torch.rand(h, d, generator=g, device="cuda") / d * 2 ** torch.randn(h, 1, generator=g, device="cuda"))
+              .bfloat16() for _ in range(2))
+    wd = (torch.rand(o, h, generator=g, device="cuda") / h).bfloat16().requires_grad_(True)
+    v = (torch.rand(n, o, generator=g, device="cuda") * 2 ** torch.randn(o, generator=g, device="cuda")).bfloat16()
+    got = torch.autograd.grad(ap.gated_feed_forward(x, wg, wu, wd), wd, v)[0].double()
+    cols = slice(0, 32)  # 256 x 32 of the gradient
+    want = torch.zeros(o, 32, device="cuda", dtype=torch.float64)
+    for r in range(0, n, 50_000):
+        rows = x[r:r + 50_000].double()
+        hid = orc.silu(rows @ wg[cols].double().T) * (rows @ wu[cols].double().T)
+        want += v[r:r + 50_000].double().T @ hid
+    assert abs(float((got[:, cols] / want - 1).mean())) < 1.2e-4 + 4.3e-5
+
+
+def test_bfloat16_gradients_of_more_rows_than_a_sweep():
+    """dX and the weights' gradients from one kernel, whose blocks each take more
+    tiles than their accumulators hold: products of one sign, so that each result
+    is off by its own rounding and the hidden values' at most, twice 2^-8 and the
+    product of both."""
+    from tidegs_b200 import appearance as ap
+
+    n, d, h, o = 5_300_000, 16, 16, 8
+    g = _gen(6)
+    x = torch.rand(n, d, generator=g, device="cuda").bfloat16()
+    wg, wu, wd = ((torch.rand(*shape, generator=g, device="cuda") / d).bfloat16() for shape in ((h, d), (h, d), (o, h)))
+    v = torch.rand(n, o, generator=g, device="cuda").bfloat16()
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    got = torch.autograd.grad(ap.gated_feed_forward(*leaves), leaves, v)
+    want = [[], 0, 0, 0]
+    deep = [w.detach().double() for w in leaves[1:]]
+    for r in range(0, n, 1_000_000):
+        v_x, *v_w = orc.gated_feed_forward_grads(x[r:r + 1_000_000].detach().double(), *deep,
+                                                 v[r:r + 1_000_000].double())
+        want[0].append(v_x)
+        want[1:] = [a + b for a, b in zip(want[1:], v_w)]
+    want[0] = torch.cat(want[0])
+    for a, e in zip(got, want):
+        assert float((a.double() / e - 1).abs().max()) <= 2.1 * HALF[torch.bfloat16]

@@ -49,6 +49,14 @@ constexpr int kChunk = 64;     // hidden values
 constexpr int kMaxTiles = 3;   // row-tile buffers
 constexpr int kMaxHid = 4;     // hidden buffers
 constexpr int kMaxSlots = 12;  // weight ring
+// Tiles whose products the accumulators of the weights' gradients take up before
+// they are added to the block's sums in memory (128: 1,024 instructions, twice
+// that with kFine). An instruction cuts off, always towards zero, what does not
+// fit the sum's 24 bits: over 300,000 rows of one slice, products of one sign
+// lost 1.8e-3 of the gradient without an end to it, 1.7e-4 with one every 256
+// tiles, 7e-5 every 128, 2e-5 every 64, where its own rounding to bf16 is 1.7e-3.
+// Every 64 costs 13 of 183 us at 200,001 rows of 128 -> 384 -> 128, every 128 none.
+constexpr int kSweep = 128;
 constexpr int kSmemBudget = 227 * 1024 - 2048;  // less alignment and barriers
 
 struct TcParams {
@@ -76,7 +84,7 @@ enum : int { kFwd = 0, kDx = 1, kDw = 2, kDxDw = 3 };
 struct TcBars {
   uint64_t xfull[kMaxTiles], xempty[kMaxTiles];
   uint64_t gfull[2], gempty[2], hfull[kMaxHid], hempty[kMaxHid];
-  uint64_t yfull[2], yempty[2], done, accfull;
+  uint64_t yfull[2], yempty[2], done, accfull, accempty;
   uint64_t wfull[kMaxSlots], wempty[kMaxSlots];
   uint32_t tmem;
 };
@@ -328,16 +336,20 @@ __device__ __forceinline__ void store_staged(const TcParams& p, int64_t tile, in
   asm volatile("bar.sync 1, %0;" ::"n"(kOut) : "memory");
 }
 
-// This block's sum of one weight gradient's chunk, out of its accumulators.
-__device__ __forceinline__ void store_partial(uint32_t acc, float* dst, int cols, bool on) {
+// One weight gradient's chunk, out of its accumulators: the block's sum in
+// memory, or (`add`) a further share of it.
+__device__ __forceinline__ void store_partial(uint32_t acc, float* dst, int cols, bool on, bool add) {
   for (int c = 0; c < cols; c += 16) {
     float v[16];
     tmem_ld(acc + c, v);
     tmem_wait_ld(v);
     if (on) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(dst + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      for (int i = 0; i < 16; i += 4) {
+        float4* to = reinterpret_cast<float4*>(dst + c + i);
+        const float4 s = add ? *to : make_float4(0.f, 0.f, 0.f, 0.f);
+        *to = make_float4(s.x + v[i], s.y + v[i + 1], s.z + v[i + 2], s.w + v[i + 3]);
+      }
     }
     __syncwarp();
   }
@@ -387,7 +399,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
         mbar_init(&bars.yfull[i], 1), mbar_init(&bars.yempty[i], kOut / 32);
       }
       for (int i = 0; i < kMaxHid; ++i) mbar_init(&bars.hfull[i], kEpi / 64), mbar_init(&bars.hempty[i], 1);
-      mbar_init(&bars.done, 2), mbar_init(&bars.accfull, 1);
+      mbar_init(&bars.done, 2), mbar_init(&bars.accfull, 1), mbar_init(&bars.accempty, kOut / 32);
       for (int i = 0; i < kMaxSlots; ++i) mbar_init(&bars.wfull[i], 1), mbar_init(&bars.wempty[i], 1);
       fence_mbar_init();
     }
@@ -531,9 +543,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
       }
     } else {
       int j = 0, t = 0, hb = 0, hphase = 0, xb = 0;
+      int left = kSweep;  // tiles of the gradients' sweep to come
       for (int it = 0; it < steps; ++it) {
         wait(&bars.hfull[hb], hphase);
         if (kRows && j == 0 && t >= p.ny) wait(&bars.yempty[(t - p.ny) & 1], (t - p.ny) >> 1);
+        if (kHasDw && left == 0) {
+          wait(&bars.accempty, t / kSweep - 1);
+          left = kSweep;
+        }
         tc_fence_after();
         const uint32_t y = yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols;
         const uint32_t h = hs + (p.nh > 1 ? hb : 0) * p.h_bytes;
@@ -548,11 +565,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
             if (want_gu)
               tc_mma_steps<8>(acc, desc_mn(from + dg_at, kBlockBytes), kStepMn,
                               desc_mn(x, kBlockBytes), kStepMn, tc_idesc(gu_cols, true, true), 8,
-                              t + part > 0);
+                              left < kSweep || part > 0);
             if (want_d)
               tc_mma_steps<8>(acc + gu_cols, desc_mn(from, kBlockBytes), kStepMn,
                               desc_mn(dy, kBlockBytes), kStepMn, tc_idesc(d_cols, true, true), 8,
-                              t + part > 0);
+                              left < kSweep || part > 0);
           }
         }
         if constexpr (kBwd && kRows) {
@@ -593,11 +610,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
         if (++j == nj) {
           if (kRows) tc_commit(&bars.yfull[t & 1]);
           if (kHasDw) tc_commit(&bars.xempty[xb]);
+          if (kHasDw && (--left == 0 || t + 1 == mine)) tc_commit(&bars.accfull);
           if (++xb == p.nx) xb = 0;
           j = 0, ++t;
         }
       }
-      if (kHasDw) tc_commit(&bars.accfull);
     }
     tc_commit(&bars.done);
     if (!tc_wait(&bars.done, 0))
@@ -676,37 +693,43 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
     }
   } else {
     const uint32_t quarter = static_cast<uint32_t>(warp & 3) << 21;
-    if constexpr (kRows) {
-      const int out = kBwd ? p.f.d : p.f.o;
-      for (int t = 0; t < mine; ++t) {
-        wait(&bars.yfull[t & 1], t >> 1);
-        tc_fence_after();
-        store_output(p, yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols + quarter,
-                     slice + static_cast<int64_t>(t) * p.slices, out, (warp & 3) * 32 + lane,
-                     p.stage_bytes ? ys : 0);
-        tc_fence_before();
-        warp_arrive(&bars.yempty[t & 1], lane);
-        if (p.stage_bytes)
-          store_staged(p, slice + static_cast<int64_t>(t) * p.slices, out, raw + (ys - smem_addr(raw)),
-                       (warp & 3) * 32 + lane);
-      }
-    }
-    if constexpr (kHasDw) {
-      // the whole sweep's end: one wait's limit for every 4096 steps
-      for (int k = 0; k < steps / 4096 && !tc_wait(&bars.accfull, 0); ++k) {
-      }
-      wait(&bars.accfull, 0);
+    const int row = (warp & 3) * 32 + lane;
+    // The gradients' accumulators at the end of a sweep (at most 1,280 steps).
+    auto drain = [&](int sweep) {
+      wait(&bars.accfull, sweep);
       tc_fence_after();
-      const int row = (warp & 3) * 32 + lane;
       for (int j = 0; j < nj; ++j) {
         float* dst = p.partial + (static_cast<int64_t>(slice) * p.nc + j0 + j) * chunk_floats(p);
         const uint32_t acc = wacc + j * (gu_cols + d_cols) + quarter;
         const bool on = (row & 63) < p.f.h - (j0 + j) * kChunk;
-        if (want_gu) store_partial(acc, dst + row * 16 * p.kd, gu_cols, on);
+        if (want_gu) store_partial(acc, dst + row * 16 * p.kd, gu_cols, on, sweep > 0);
         if (want_d && row < 64)
-          store_partial(acc + gu_cols, dst + 128 * 16 * p.kd + row * 16 * p.ko, d_cols, on);
+          store_partial(acc + gu_cols, dst + 128 * 16 * p.kd + row * 16 * p.ko, d_cols, on, sweep > 0);
       }
       tc_fence_before();
+      warp_arrive(&bars.accempty, lane);
+    };
+    // Output tiles [begin, end).
+    auto rows = [&](int begin, int end) {
+      const int out = kBwd ? p.f.d : p.f.o;
+      for (int t = begin; t < end; ++t) {
+        wait(&bars.yfull[t & 1], t >> 1);
+        tc_fence_after();
+        store_output(p, yacc + (p.ny == 2 ? t & 1 : 0) * p.ycols + quarter,
+                     slice + static_cast<int64_t>(t) * p.slices, out, row, p.stage_bytes ? ys : 0);
+        tc_fence_before();
+        warp_arrive(&bars.yempty[t & 1], lane);
+        if (p.stage_bytes)
+          store_staged(p, slice + static_cast<int64_t>(t) * p.slices, out, raw + (ys - smem_addr(raw)), row);
+      }
+    };
+    if constexpr (kHasDw) {
+      for (int t = 0; t < mine; t += kSweep) {
+        if constexpr (kRows) rows(t, min(t + kSweep, mine));
+        drain(t / kSweep);
+      }
+    } else {
+      rows(0, mine);
     }
   }
   __syncwarp();
