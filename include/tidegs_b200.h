@@ -855,7 +855,8 @@ typedef struct {
   int32_t o;           /* 1..256 */
   int32_t dtype;       /* TGS_F32 or TGS_BF16, of every tensor */
   float* scratch;      /* tgs_ffn_scratch_floats(...) floats, 16-byte aligned */
-  int32_t* err;        /* error word (a wait that ran out), or NULL */
+  int32_t* err;        /* four words, a wait that ran out; memory of the device or
+                          page-locked memory of the host; or NULL */
 } TgsFfnArgs;
 
 /* y = (silu(x w_gate^T) * (x w_up^T)) w_down^T. bf16: one kernel (a second one

@@ -224,3 +224,84 @@ def test_bfloat16_gradients_of_more_rows_than_a_sweep():
     want[0] = torch.cat(want[0])
     for a, e in zip(got, want):
         assert float((a.double() / e - 1).abs().max()) <= 2.1 * HALF[torch.bfloat16]
+
+
+# --- waits that ran out -----------------------------------------------------------------
+
+def test_the_next_call_tells_of_a_wait_that_ran_out():
+    """The error word lies where the host reads it without waiting: a call on
+    the device that follows such a kernel raises, once (the word is set by hand)."""
+    from tidegs_b200 import appearance as ap
+
+    *ins, v = _ffn_inputs(10, 16, 16, 16, torch.bfloat16)
+    x = ins[0].requires_grad_(True)
+    y = ap.gated_feed_forward(*ins)
+    word = ap._err_words[x.device]
+    assert not word.is_cuda and word.is_pinned()
+    word[0] = 4
+    with pytest.raises(RuntimeError, match="timed out"):
+        ap.gated_feed_forward(*ins)
+    ap.gated_feed_forward(*ins)
+    word[0] = 4
+    with pytest.raises(RuntimeError, match="timed out"):
+        torch.autograd.grad(y, x, v, retain_graph=True)
+    torch.autograd.grad(y, x, v)
+    word[0] = 4
+    with pytest.raises(RuntimeError, match="timed out"):
+        ap.check()
+    ap.check()
+
+
+def test_kernels_reach_the_error_word():
+    """Another kernel that reports by the same function (an id past a bitmap's
+    end, which it skips) writes into it."""
+    from tidegs_b200 import _lib
+    from tidegs_b200 import appearance as ap
+
+    device = torch.device("cuda", torch.cuda.current_device())
+    word = ap._err_word(device)
+    bits, ids = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([3, 5, 64, 7], device="cuda")
+    _lib.call("tgs_bitmap_set", bits.data_ptr(), 64, ids.data_ptr(), 4, word.data_ptr(),
+              torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(RuntimeError, match="index 2"):
+        ap.check()
+    assert not word.any() and bits.tolist() == [8 + 32 + 128, 0]
+
+
+def test_a_first_call_under_capture_has_its_error_word():
+    _child("""
+import torch
+from tidegs_b200 import appearance as ap
+x, w = torch.randn(300, 32, device="cuda").bfloat16(), torch.randn(32, 32, device="cuda").bfloat16()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ap.gated_feed_forward(x, w, w, w)
+word = ap._err_words[x.device]
+graph.replay()
+ap.check()
+assert torch.equal(y, ap.gated_feed_forward(x, w, w, w))
+word[0] = 4
+try:
+    ap.check()
+except RuntimeError as e:
+    assert "timed out" in str(e)
+else:
+    raise AssertionError("not told")
+""")
+
+
+def test_first_calls_from_several_threads_share_one_error_word():
+    _child("""
+import threading, torch
+from tidegs_b200 import appearance as ap
+device = torch.device("cuda", 0)
+torch.zeros(1, device=device)
+gate, got = threading.Barrier(8), []
+def run():
+    gate.wait()
+    got.append(ap._err_word(device).data_ptr())
+threads = [threading.Thread(target=run) for _ in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert len(got) == 8 and len(set(got)) == 1 and got[0] == ap._err_words[device].data_ptr(), got
+""")

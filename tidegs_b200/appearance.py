@@ -21,7 +21,9 @@ Kernels: tgs_layer_norm_fwd/bwd, tgs_ffn_fwd/bwd, tgs_dropout
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import operator
+import threading
 from typing import Dict, Optional, Tuple, Union
 
 import torch
@@ -179,31 +181,46 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
 # --- gated feed-forward block --------------------------------------------------
 
+# A device's error word, in page-locked memory: kernels write it, the host reads
+# it without waiting for them.
 _err_words: Dict[torch.device, torch.Tensor] = {}
+_err_values: Dict[torch.device, ctypes.Array] = {}
+_err_lock = threading.Lock()
 
 
-def _err_word(device: torch.device) -> Optional[torch.Tensor]:
-    """The device's error word (none while a capture runs that came first)."""
+def _err_word(device: torch.device) -> torch.Tensor:
     word = _err_words.get(device)
-    if word is None and not torch.cuda.is_current_stream_capturing():
-        word = _err_words[device] = torch.zeros(4, dtype=torch.int32, device=device)
+    if word is None:
+        with _err_lock, torch.inference_mode(False):
+            word = _err_words.get(device)
+            if word is None:
+                word = torch.zeros(4, dtype=torch.int32, device="cpu", pin_memory=True)
+                _err_values[device] = (ctypes.c_int32 * 4).from_address(word.data_ptr())
+                _err_words[device] = word
     return word
+
+
+def _raise_recorded(device: torch.device) -> None:
+    """Raises, once, what a kernel on `device` has recorded."""
+    values = _err_values.get(device)
+    if values is not None and values[0]:
+        problem = _lib.decode_device_error(list(values))
+        _err_words[device].zero_()
+        raise RuntimeError(f"[gated_feed_forward] in an earlier call on {device}: {problem}")
 
 
 def check(device=None) -> None:
     """Raises if a bounded wait inside an earlier gated_feed_forward kernel on
     `device` (default: the current one) ran out, which leaves that call's
-    results undefined. Waits for the device."""
+    results undefined. Waits for the device. (A later gated_feed_forward call,
+    or backward, raises too, without waiting: as soon as the host can know.
+    Either tells once.)"""
     device = torch.device("cuda" if device is None else device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    word = _err_words.get(device)
-    if word is None:
-        return
-    torch.cuda.synchronize(device)
-    problem = _lib.decode_device_error(word.cpu().tolist())
-    if problem is not None:
-        raise RuntimeError(f"[gated_feed_forward] {problem}")
+    if device in _err_words:
+        torch.cuda.synchronize(device)
+        _raise_recorded(device)
 
 
 def _ffn_rows(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -227,13 +244,14 @@ def _ffn_stride(t: torch.Tensor) -> int:
 
 def _ffn_args(x, w_gate, w_up, w_down, backward: bool):
     """(arguments, scratch tensor or None); on the tensors' device."""
+    _raise_recorded(x.device)
     a = _lib.FfnArgs()
     a.x, a.w_gate = x.data_ptr(), w_gate.data_ptr()
     a.w_up, a.w_down = w_up.data_ptr(), w_down.data_ptr()
     a.n, a.x_stride = x.shape[0], _ffn_stride(x)
     a.d, a.h, a.o = int(w_gate.shape[1]), int(w_gate.shape[0]), int(w_down.shape[0])
     a.dtype = _lib.DTYPES[x.dtype]
-    a.err = _lib.ptr(_err_word(x.device))
+    a.err = _err_word(x.device).data_ptr()
     words = _lib.load().tgs_ffn_scratch_floats(a.n, a.d, a.h, a.o, a.dtype, int(backward))
     scratch = torch.empty(words, dtype=torch.float32, device=x.device) if words else None
     a.scratch = _lib.ptr(scratch)
@@ -282,8 +300,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     """(silu(x w_gate^T) * (x w_up^T)) w_down^T for rows x [..., D]; w_gate
     and w_up [H, D], w_down [O, H]; D and O up to 256, H up to 4096; every
     tensor float32 or every tensor bfloat16. Differentiable in all four; the
-    hidden values are not kept: the backward computes them again. `check` tells
-    whether a kernel gave up waiting.
+    hidden values are not kept: the backward computes them again. Raises if an
+    earlier call's kernel gave up waiting (see `check`).
 
     bfloat16: the hidden values, and their gradients, are rounded to bfloat16
     between the products (calls of at most 128 rows per SM: to two bfloat16
