@@ -860,9 +860,8 @@ typedef struct {
 } TgsFfnArgs;
 
 /* y = (silu(x w_gate^T) * (x w_up^T)) w_down^T. bf16: one kernel (a second one
- * lays out weights that do not fit shared memory), hidden values rounded to
- * bf16 (to two bf16 parts in calls of at most 128 rows per SM). fp32: one
- * kernel, or, from 12,288 multiply-adds a row on, products on the tensor cores
+ * lays out weights that do not fit shared memory), hidden values in two bf16
+ * parts (in the backward of more than 18,944 rows, one). fp32: one kernel, or, from 12,288 multiply-adds a row on, products on the tensor cores
  * with a batch's hidden values in scratch. The error word tells of a wait that
  * ran out (TGS_DEV_WAIT_TIMEOUT); the kernels run whatever it holds. */
 TGS_API int tgs_ffn_fwd(const TgsFfnArgs* args, void* stream);

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from oracle import appearance as orc
-from test_gpu_appearance import HALF, _ffn_check, _ffn_inputs, _gen
+from test_gpu_appearance import HALF, _far, _ffn_check, _ffn_expect, _ffn_inputs, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -305,3 +305,36 @@ threads = [threading.Thread(target=run) for _ in range(8)]
 [t.join() for t in threads]
 assert len(got) == 8 and len(set(got)) == 1 and got[0] == ap._err_words[device].data_ptr(), got
 """)
+
+
+# --- a row's result is its own --------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d,h,o", [(32, 64, 3), (64, 128, 48), (128, 384, 128), (200, 40, 30), (256, 512, 256)])
+def test_a_row_gives_the_same_bits_in_calls_of_any_size(dtype, d, h, o):
+    """A Gaussian's color does not depend on how many others the call holds; its
+    gradient, in bfloat16, only on whether they are more than 18,944."""
+    from tidegs_b200 import appearance as ap
+
+    x, wg, wu, wd, v = _ffn_inputs(40000, d, h, o, dtype)
+    ws = [w.requires_grad_(True) for w in (wg, wu, wd)]
+
+    def run(k, weights):
+        rows = x[:k].detach().requires_grad_(True)
+        y = ap.gated_feed_forward(rows, *weights)
+        return y.detach(), torch.autograd.grad(y, [rows, *(w for w in weights if w.requires_grad)], v[:k])[0]
+
+    whole, most = run(40000, ws), run(18944, ws)
+    for k in (1, 200, 18944, 18945, 30001):
+        for weights in (ws, [w.detach() for w in ws]):
+            y, v_x = run(k, weights)
+            assert torch.equal(y, whole[0][:k])
+            assert torch.equal(v_x, (whole if k > 18944 or dtype == torch.float32 else most)[1][:k])
+
+
+@pytest.mark.parametrize("n,d,h,o", [(18945, 35, 96, 3), (20011, 64, 128, 48), (50000, 145, 72, 9), (30000, 256, 512, 256)])
+def test_large_bfloat16_calls_round_their_outputs_once(n, d, h, o):
+    from tidegs_b200 import appearance as ap
+
+    *ins, v = _ffn_inputs(n, d, h, o, torch.bfloat16, 3)
+    _far(ap.gated_feed_forward(*ins), _ffn_expect(*ins, v, torch.bfloat16, parts=2)["y"], "y")

@@ -303,12 +303,16 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     hidden values are not kept: the backward computes them again. Raises if an
     earlier call's kernel gave up waiting (see `check`).
 
-    bfloat16: the hidden values, and their gradients, are rounded to bfloat16
-    between the products (calls of at most 128 rows per SM: to two bfloat16
-    parts, 16 bits). float16 is refused: the hidden products leave its
-    range long before their inputs do. float32: products of 32 bits; blocks of
-    12,288 multiply-adds a row and more keep a batch's hidden values in scratch
-    memory, take an infinity for NaN, and lose bits of values below 2^-100."""
+    A row's output is the same in calls of any number of rows.
+
+    bfloat16: the hidden values are kept in two bfloat16 parts, 16 bits, between
+    the products (one past bfloat16's range gives NaN). The backward rounds
+    them, and their gradients, to one part in calls of more than 18,944 rows.
+    float16 is refused: the hidden products leave its range long before their
+    inputs do. float32: products of 32 bits; blocks of 12,288 multiply-adds a row
+    and more keep a batch's hidden values in scratch memory, take an infinity
+    (or a value that rounds to one in bfloat16, from 3.396e38 on) for NaN, and
+    lose bits of values below 2^-100."""
     who = "gated_feed_forward"
     if w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_down.dim() != 2 \
             or w_down.shape[1] != w_gate.shape[0]:

@@ -18,9 +18,13 @@
 // and as MN-major operand of the other.
 //
 // Rounding the hidden values to bf16 adds as much error to the results as
-// rounding those does, 0.0024 of a result in place of 0.0017. A call of at most one
-// tile per SM, whose time is that of its launches, keeps them in two bf16 parts
-// (kFine) instead: 0.0017, and as long.
+// rounding those does, 0.0024 of a result in place of 0.0017. The forward keeps
+// them in two bf16 parts (kFine), for 5 to 12 % of its time, so that a row's
+// output is 0.0017 off and the same in calls of any size. In the backward two
+// parts take up to twice as long (2,097,152 rows of 64 -> 128 -> 48: 830 us
+// against 400; 1,500 of 256 -> 4096 -> 256: 645 against 370; 1,500 of 32 -> 64
+// -> 3: 127 against 122, most of it the host's), so calls of up to kFineRows
+// rows have them and larger ones keep one part.
 //
 // Bound: at 64 -> 128 -> 48 the special-function unit (69 % busy) and waits
 // between the roles: 2,097,152 rows forward 170 us (2.8 TB/s), backward in one
@@ -57,6 +61,9 @@ constexpr int kMaxSlots = 12;  // weight ring
 // tiles, 7e-5 every 128, 2e-5 every 64, where its own rounding to bf16 is 1.7e-3.
 // Every 64 costs 13 of 183 us at 200,001 rows of 128 -> 384 -> 128, every 128 none.
 constexpr int kSweep = 128;
+// Rows of a call whose backward keeps hidden values in two parts: a tile for
+// each SM of a B200, but the same number everywhere.
+constexpr int kFineRows = 148 * kTile;
 constexpr int kSmemBudget = 227 * 1024 - 2048;  // less alignment and barriers
 
 struct TcParams {
@@ -228,7 +235,7 @@ __device__ __forceinline__ void round_pair(float a, float b, uint32_t& hi, uint3
 // value. One reciprocal for two values, 1 / a = b / (a b), saves a quarter of
 // them but costs as much again in products and moves: 196 against 168 us for
 // 2,097,152 rows of 64 -> 128 -> 48, and 168 with it for every second pair.
-template <bool kFine, int kW>
+template <int kW>
 __device__ __forceinline__ void gate(const float (&g)[kW], const float (&u)[kW],
                                      uint32_t (&h)[kW / 2], uint32_t (&lo)[kW / 2]) {
 #pragma unroll
@@ -237,7 +244,7 @@ __device__ __forceinline__ void gate(const float (&g)[kW], const float (&u)[kW],
     float a, b;
     one_plus_exp(g2).get(a, b);
     (g2 * F2(fast_rcp(a), fast_rcp(b)) * F2(u[i], u[i + 1])).get(a, b);
-    round_pair<kFine>(a, b, h[i / 2], lo[i / 2]);
+    round_pair<true>(a, b, h[i / 2], lo[i / 2]);
   }
 }
 
@@ -444,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
       // whole 16-steps of the chunk's hidden values
       const int cols = (min(kChunk, p.f.h - (j0 + j) * kChunk) + 15) & ~15;
       constexpr int kParts = kBwd ? 3 : 2;  // G, U, dH
-      constexpr int kW = kHasDw || kFine ? 8 : 16;  // what the registers hold
+      constexpr int kW = kHasDw || (kFine && kBwd) ? 8 : 16;  // what the registers hold
       constexpr int kTurns = kChunk / kW / 2;
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) ffn_tc_kernel(const __grid_cons
           if constexpr (kBwd) {
             gate_backward<kHasDw, kFine>(v[0], v[1], v[kParts - 1], h, dg, du, h_lo, dg_lo, du_lo);
           } else {
-            gate<kFine>(v[0], v[1], h, h_lo);
+            gate(v[0], v[1], h, h_lo);
           }
           if (kMode == kFwd || (kHasDw && want_d)) store_granule(hbuf, row, q, h);
           if (kBwd && want_gu) {
@@ -789,14 +796,14 @@ uint32_t pow2_cols(uint32_t c) {
   return p;
 }
 
-TcParams tc_params(const FfnParams& f) {
+TcParams tc_params(const FfnParams& f, bool bwd) {
   TcParams p{};
   p.f = f;
   p.kd = ceil_div(f.d, 16), p.ko = ceil_div(f.o, 16);
   p.cd = ceil_div(f.d, 64), p.co = ceil_div(f.o, 64), p.nc = ceil_div(f.h, kChunk);
   p.tiles = ceil_div<int64_t>(f.n, kTile);
   p.cpc = p.nc, p.groups = 1;
-  p.fine = p.tiles <= sm_count();
+  p.fine = !bwd || f.n <= kFineRows;
   return p;
 }
 
@@ -927,11 +934,11 @@ struct BwdPlan {
 
 BwdPlan plan_backward(const FfnParams& f, bool dx, bool dw) {
   BwdPlan b{};
-  b.rows = b.weights = tc_params(f);
+  b.rows = b.weights = tc_params(f, true);
   b.both = dx && dw && !b.weights.fine && plan_weights(b.weights, true);
   bool packed = false;
   if (dw && !b.both) {
-    b.weights = tc_params(f);
+    b.weights = tc_params(f, true);
     plan_weights(b.weights, false);
     packed |= !b.weights.resident;
   }
@@ -974,20 +981,20 @@ int make_row_map(CUtensorMap* map, const void* base, int64_t rows, int cols, int
 }
 
 int ffn_tc_forward(const FfnParams& f, cudaStream_t s) {
-  TcParams p = tc_params(f);
+  TcParams p = tc_params(f, false);
   plan_rows(p, false);
   if (!p.resident) {
     p.packed = reinterpret_cast<const uint8_t*>(f.scratch);
     if (int rc = pack_weights(p, reinterpret_cast<uint8_t*>(f.scratch), s)) return rc;
   }
-  return p.fine ? launch_tc<kFwd, true>(p, s) : launch_tc<kFwd>(p, s);
+  return launch_tc<kFwd, true>(p, s);
 }
 
 int64_t ffn_tc_scratch_floats(int64_t n, int d, int h, int o, bool backward) {
   FfnParams f{};
   f.n = n, f.d = d, f.h = h, f.o = o;
   if (!backward) {
-    TcParams p = tc_params(f);
+    TcParams p = tc_params(f, false);
     plan_rows(p, false);
     return p.resident ? 0 : weight_bytes(p, p.nc) / 4;
   }
