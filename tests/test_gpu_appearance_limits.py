@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from oracle import appearance as orc
-from test_gpu_appearance import HALF, _far, _ffn_check, _ffn_expect, _ffn_inputs, _gen
+from test_gpu_appearance import HALF, TYPES, U, _far, _ffn_check, _ffn_expect, _ffn_inputs, _gen, _norm_inputs, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -332,9 +332,106 @@ def test_a_row_gives_the_same_bits_in_calls_of_any_size(dtype, d, h, o):
             assert torch.equal(v_x, (whole if k > 18944 or dtype == torch.float32 else most)[1][:k])
 
 
-@pytest.mark.parametrize("n,d,h,o", [(18945, 35, 96, 3), (20011, 64, 128, 48), (50000, 145, 72, 9), (30000, 256, 512, 256)])
+@pytest.mark.parametrize("n,d,h,o", [(18945, 35, 96, 3), (20011, 64, 128, 48), (50000, 145, 72, 9),
+                                     (30000, 256, 512, 256)])
 def test_large_bfloat16_calls_round_their_outputs_once(n, d, h, o):
     from tidegs_b200 import appearance as ap
 
     *ins, v = _ffn_inputs(n, d, h, o, torch.bfloat16, 3)
     _far(ap.gated_feed_forward(*ins), _ffn_expect(*ins, v, torch.bfloat16, parts=2)["y"], "y")
+
+
+# --- every row counts -------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d,h,o", [(60000, 256, 192, 256), (50000, 130, 129, 200), (60000, 64, 40, 64),
+                                     (40003, 64, 128, 48)])
+def test_every_tile_of_rows_enters_the_weight_gradients(dtype, n, d, h, o):
+    """Row r's inputs are zero but in column (r / 128) % D, its gradients but in
+    column (r / 128) % O: a column of the weights' gradients sums few rows, and
+    its bound is those rows', so that a lost or doubled tile is seen."""
+    from tidegs_b200 import appearance as ap
+
+    x, wg, wu, wd, v = _ffn_inputs(n, d, h, o, dtype)
+    tile = torch.arange(n, device="cuda") // 128
+    x = x.abs() + 0.5
+    v = v.abs() + 0.05
+    x = torch.where((tile % d)[:, None] == torch.arange(d, device="cuda"), x, 0).to(dtype)
+    v = torch.where((tile % o)[:, None] == torch.arange(o, device="cuda"), v, 0).to(dtype)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    _, got_g, got_u, got_d = torch.autograd.grad(ap.gated_feed_forward(*leaves), leaves, v)
+    args = [t.detach() for t in leaves]
+    for k in range(max(d, o)):
+        if k < d:
+            rows = (tile % d == k).nonzero()[:, 0]
+            want = _ffn_expect(args[0][rows], *args[1:], v[rows], dtype)
+            _far(got_g[:, k], _column(want["v_w_gate"], k), f"v_w_gate, column {k}")
+            _far(got_u[:, k], _column(want["v_w_up"], k), f"v_w_up, column {k}")
+        if k < o:
+            rows = (tile % o == k).nonzero()[:, 0]
+            want = _ffn_expect(args[0][rows], *args[1:], v[rows], dtype)["v_w_down"]
+            _far(got_d[k], _column(want.T, k), f"v_w_down, row {k}")
+
+
+def _column(want, k):
+    return type(want)(want.val[:, k], want.err[:, k])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,c", [(50001, 768), (50001, 59), (30000, 64), (20000, 1025)])
+def test_every_row_enters_the_norm_gradients(dtype, n, c):
+    """Row r's gradient is zero but in column (r / 8) % C."""
+    from tidegs_b200 import appearance as ap
+
+    x, w, b, v = _norm_inputs(n, c, dtype, torch.float32)
+    on = (torch.arange(n, device="cuda") // 8 % c)[:, None] == torch.arange(c, device="cuda")
+    v = torch.where(on, v.abs() + 0.05, 0).to(dtype)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    _, got_w, got_b = torch.autograd.grad(ap.layer_norm(*leaves), leaves, v)
+    # the sums' bounds by the rows that count: zeros add exactly
+    most = int(on.sum(0).max())
+    x64, v64 = x.detach().double(), v.double()
+    dev = x64 - x64.mean(1, keepdim=True)
+    std = torch.sqrt((dev * dev).mean(1, keepdim=True) + 1e-5)
+    z = dev / std
+    unit = (c + 16) * U * (1 + x64.abs().amax(1, keepdim=True) / std)
+    want_w, want_b = (v64 * z).sum(0), v64.sum(0)
+    z_err = unit * (1 + z.abs())
+    err_w = (v64 * z_err).sum(0) + (most + 4) * U * (v64 * (z.abs() + z_err)).sum(0)
+    assert bool(((got_w.double() - want_w).abs() <= err_w + HALF[torch.float32] * want_w.abs()).all())
+    assert bool(((got_b.double() - want_b).abs() <= (most + 4) * U * want_b).all())
+
+
+@pytest.mark.parametrize("n,d,h,o", [(3000, 256, 512, 256), (60000, 128, 256, 128), (5000, 35, 96, 3)])
+def test_float32_errors_as_a_whole(n, d, h, o):
+    """The 2-norm of the error. A result's sums run through H (or D, or n)
+    terms; on the fp32 pipes each addition is off by at most 2^-24 of the
+    partial sum, at random: sqrt(K) 2^-24 / sqrt(3) of the terms' spread, as
+    large as the result's: 4e-7 at 512. On the tensor cores a piece of 64 loses up
+    to 8 x 2^-24 in the additions of its largest products and 2^-24 more in those
+    of the smaller ones, 5.4e-7 at most. Three such products follow one another,
+    each with its own errors: sqrt(3) x 5.4e-7 = 9.3e-7."""
+    from tidegs_b200 import appearance as ap
+
+    *ins, v = _ffn_inputs(n, d, h, o, torch.float32)
+    leaves = [t.requires_grad_(True) for t in ins]
+    y = ap.gated_feed_forward(*leaves)
+    got = (y.detach(), *torch.autograd.grad(y, leaves, v))
+    deep = [t.detach().double() for t in ins]
+    want = (orc.gated_feed_forward(*deep), *orc.gated_feed_forward_grads(*deep, v.double()))
+    for a, e in zip(got, want):
+        assert float((a.double() - e).norm() / e.norm()) < 1e-6
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dropout_of_whole_rows_with_strides(dtype):
+    from tidegs_b200 import appearance as ap
+
+    wide = _rand(_gen(6), 90, 72, dtype=dtype)
+    ids = torch.arange(180, device="cuda")[::2] * 7 + 2 ** 35
+    for x in (wide[:, 8:40], wide[:, 1:34], wide[::2, :32], wide[:, ::2], wide[:40].T, wide[:1].expand(90, 72)):
+        who = ids[:x.shape[0]]
+        got = ap.dropout(x, 0.4, 8, offset=2, ids=who, per_row=True)
+        assert torch.equal(got, ap.dropout(x.contiguous(), 0.4, 8, offset=2, ids=who.contiguous(), per_row=True))
+        kept = torch.from_numpy(orc.dropout_keep(x.shape[0], 1, 0.4, 8, 2, who.cpu().numpy())).cuda()
+        assert torch.equal(got != 0, kept & (x != 0))
