@@ -93,6 +93,10 @@ TGS_API int tgs_version(void);
  * to len). Returns the full message length. */
 TGS_API int tgs_last_error(char* buf, size_t len);
 
+/* Kernels launched by the calling thread's last call of an entry point whose
+ * number depends on its arguments: tgs_layer_norm_bwd, tgs_ffn_fwd/bwd. */
+TGS_API int32_t tgs_launches(void);
+
 /* ------------------------------------------------------------------------ */
 /* GPU-resident Adam                                                         */
 /* Replaces: strategies/tide_engine/gpu_resident_optimizer.py                */

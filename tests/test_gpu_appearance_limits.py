@@ -435,3 +435,42 @@ def test_dropout_of_whole_rows_with_strides(dtype):
         assert torch.equal(got, ap.dropout(x.contiguous(), 0.4, 8, offset=2, ids=who.contiguous(), per_row=True))
         kept = torch.from_numpy(orc.dropout_keep(x.shape[0], 1, 0.4, 8, 2, who.cpu().numpy())).cuda()
         assert torch.equal(got != 0, kept & (x != 0))
+
+
+# --- accounts -----------------------------------------------------------------------
+
+def test_launches_are_counted():
+    """The kernels that a call launched, by the plans of the different forms."""
+    from tidegs_b200 import _lib
+    from tidegs_b200 import appearance as ap
+
+    def count(f):
+        before = _lib.launch_counter["kernels"]
+        f()
+        return _lib.launch_counter["kernels"] - before
+
+    def ffn(n, d, h, o, dtype, grads):
+        *ins, v = _ffn_inputs(n, d, h, o, dtype)
+        leaves = [t.requires_grad_(grads in ("all", k)) for k, t in zip(("x", "", "", ""), ins)]
+        if not grads:
+            with torch.no_grad():
+                return count(lambda: ap.gated_feed_forward(*leaves))
+        y = ap.gated_feed_forward(*leaves)
+        return count(lambda: torch.autograd.grad(y, [t for t in leaves if t.requires_grad], v))
+
+    f32, b16 = torch.float32, torch.bfloat16
+    assert ffn(100, 35, 96, 3, f32, "") == 1
+    assert ffn(100, 35, 96, 3, f32, "x") == 1
+    assert ffn(100, 35, 96, 3, f32, "all") == 3            # dX, weights, their sum
+    assert ffn(100, 128, 256, 128, f32, "") == 5           # three splits, hidden values, output
+    assert ffn(100, 128, 256, 128, f32, "all") == 8        # four splits, hidden, dX, weights, their sum
+    assert ffn(100, 64, 128, 48, b16, "") == 1
+    assert ffn(100, 256, 512, 256, b16, "") == 2           # weights laid out before
+    assert ffn(100, 256, 512, 256, b16, "all") == 4        # and dX, weights, their sum
+    x, w, b, v = _norm_inputs(50, 40, f32, f32)
+    x.requires_grad_(True)
+    y = ap.layer_norm(x, w, b)
+    assert count(lambda: torch.autograd.grad(y, x, v, retain_graph=True)) == 1
+    w.requires_grad_(True)
+    y = ap.layer_norm(x, w, b)
+    assert count(lambda: torch.autograd.grad(y, (x, w), v)) == 2

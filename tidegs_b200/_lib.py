@@ -230,6 +230,7 @@ class DropoutArgs(C.Structure):
 SIGNATURES = {
     "tgs_version": (C.c_int, []),
     "tgs_last_error": (C.c_int, [C.c_char_p, C.c_size_t]),
+    "tgs_launches": (_i32, []),
     "tgs_resident_adam_count": (C.c_int, [C.POINTER(ResidentCountArgs), _vp]),
     "tgs_resident_adam_apply": (C.c_int, [C.POINTER(ResidentAdamArgs), _vp]),
     "tgs_selective_adam": (C.c_int, [C.POINTER(DenseArgs), _vp]),
@@ -351,9 +352,10 @@ KERNELS_PER_CALL = {
     # iota + the library radix sort and scan (their kernel counts depend on
     # the library version and are not counted here)
     "tgs_isect_depth_order": 1, "tgs_isect_sort_tiles": 0,
-    "tgs_layer_norm_fwd": 1, "tgs_layer_norm_bwd": 2, "tgs_ffn_fwd": 1, "tgs_ffn_bwd": 2,
-    "tgs_dropout": 1, "tgs_align_rows": 1,
+    "tgs_layer_norm_fwd": 1, "tgs_dropout": 1, "tgs_align_rows": 1,
 }
+# Entry points that launch by their arguments; the library counts for them.
+COUNTED_CALLS = frozenset(("tgs_layer_norm_bwd", "tgs_ffn_fwd", "tgs_ffn_bwd"))
 launch_counter = {"kernels": 0}
 
 
@@ -375,7 +377,8 @@ def call(name: str, *args) -> None:
         status = getattr(lib, name)(*args)
     if status != 0:
         raise RuntimeError(f"[tidegs_b200] {name} failed (status {status}): {last_error()}")
-    launch_counter["kernels"] += KERNELS_PER_CALL.get(name, 0)
+    launch_counter["kernels"] += (lib.tgs_launches() if name in COUNTED_CALLS
+                                  else KERNELS_PER_CALL.get(name, 0))
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

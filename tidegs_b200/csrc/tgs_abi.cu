@@ -10,6 +10,7 @@ namespace tgs {
 
 namespace {
 thread_local char g_last_error[1024] = {0};
+thread_local int32_t g_launches = 0;
 }  // namespace
 
 void set_error(const char* fmt, ...) {
@@ -18,6 +19,8 @@ void set_error(const char* fmt, ...) {
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
   va_end(ap);
 }
+
+int32_t& launches() { return g_launches; }
 
 int sm_count() {
   static int cached[64] = {0};
@@ -35,6 +38,8 @@ int sm_count() {
 }  // namespace tgs
 
 extern "C" int tgs_version(void) { return TGS_ABI_VERSION; }
+
+extern "C" int32_t tgs_launches(void) { return tgs::launches(); }
 
 extern "C" int tgs_last_error(char* buf, size_t len) {
   const size_t n = strlen(tgs::g_last_error);

@@ -18,6 +18,10 @@ namespace tgs {
 // ---------------------------------------------------------------------------
 void set_error(const char* fmt, ...);
 
+// Kernels that the calling thread launched since an entry point that counts
+// them (tgs_launches) set this to zero.
+int32_t& launches();
+
 #define TGS_CHECK_ARG(cond, ...)              \
   do {                                        \
     if (!(cond)) {                            \
@@ -38,6 +42,7 @@ void set_error(const char* fmt, ...);
 
 #define TGS_LAUNCH_CHECK()                                                  \
   do {                                                                      \
+    ++::tgs::launches();                                                    \
     cudaError_t e_ = cudaGetLastError();                                    \
     if (e_ != cudaSuccess) {                                                \
       ::tgs::set_error("kernel launch failed: %s (%s:%d)",                 \

@@ -507,6 +507,7 @@ extern "C" int64_t tgs_ffn_scratch_floats(int64_t n, int32_t d, int32_t h, int32
 }
 
 extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
+  launches() = 0;
   if (int rc = check_ffn(a, "tgs_ffn_fwd")) return rc;
   if (a->n == 0) return TGS_OK;
   TGS_CHECK_ARG(a->y != nullptr, "tgs_ffn_fwd: NULL pointer");
@@ -522,6 +523,7 @@ extern "C" int tgs_ffn_fwd(const TgsFfnArgs* a, void* stream) {
 }
 
 extern "C" int tgs_ffn_bwd(const TgsFfnBwdArgs* b, void* stream) {
+  launches() = 0;
   TGS_CHECK_ARG(b != nullptr, "tgs_ffn_bwd: args is NULL");
   const TgsFfnArgs& a = b->fwd;
   if (int rc = check_ffn(&a, "tgs_ffn_bwd")) return rc;

@@ -417,6 +417,7 @@ extern "C" int64_t tgs_layer_norm_scratch_floats(int64_t n, int32_t c) {
 }
 
 extern "C" int tgs_layer_norm_bwd(const TgsLayerNormBwdArgs* b, void* stream) {
+  launches() = 0;
   TGS_CHECK_ARG(b != nullptr, "tgs_layer_norm_bwd: args is NULL");
   const TgsLayerNormArgs& a = b->fwd;
   if (int rc = check_norm(&a, "tgs_layer_norm_bwd")) return rc;
