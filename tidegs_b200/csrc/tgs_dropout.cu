@@ -9,10 +9,14 @@
 // Dropped values become zero by selection, so NaN or infinity there is gone.
 //
 // Bound: HBM for 32-bit rows of several columns (one generator call serves
-// four of them); the generator's 20 wide products per call weigh as much as
-// the traffic for 16-bit rows and for single columns. Measured: 1,048,576 rows
-// of 64 fp32 97 us (5.6 TB/s, 87 % of the copy rate), of 64 bf16 82 us (3.4
-// TB/s), 4,194,304 rows of one fp32 value by ids 27 us.
+// four of them): 1,048,576 rows of 64 fp32 97 us (5.5 TB/s, 86 % of the copy
+// rate). 16-bit rows: the generator, whose wide products keep the half of the
+// multiply-add units that has them 64 % busy, the logical operations the other
+// arithmetic 54 %, with registers for 5.5 warps to a scheduler (the four items
+// in flight) between whose loads that work stands: of 64 bf16 82 us (3.3 TB/s).
+// Single columns have a generator call each: 4,194,304 rows of one fp32 value
+// by ids 27 us. With per_row every item of a row draws its word again: of 64
+// fp32 91 us, of 64 bf16 59.
 #include "tgs_common.cuh"
 #include "tgs_vec.cuh"
 

@@ -26,10 +26,11 @@
 // -> 3: 127 against 122, most of it the host's), so calls of up to kFineRows
 // rows have them and larger ones keep one part.
 //
-// Bound: at 64 -> 128 -> 48 the special-function unit (69 % busy) and waits
-// between the roles: 2,097,152 rows forward 170 us (2.8 TB/s), backward in one
-// kernel 393 us; at 256 -> 512 -> 256 the matrix instructions: 400,000 rows
-// forward 335 us, 0.94 PFLOP/s, 55 % of the measured rate.
+// Bound: at 64 -> 128 -> 48 the special-function unit (65 % busy) and waits
+// between the roles: 2,097,152 rows forward 192 us (2.4 TB/s), backward in one
+// kernel 400 us; at 256 -> 512 -> 256 the matrix instructions (a third of the
+// forward's are those of the second parts): 400,000 rows forward 359 us, 0.88
+// PFLOP/s of the block's own products, 52 % of the measured rate.
 //
 // Weights stay in shared memory where they fit (then the blocks lay them out
 // themselves); else a small kernel lays them out once per call and they
@@ -195,8 +196,9 @@ struct Waits {
   }
 };
 
-// One arrival for the warp, after all of its lanes have come here (an arrival
-// per thread takes as long as the activation: they are counted one by one).
+// One arrival for the warp, after all of its lanes have come here (an arrival of
+// each thread takes the same time: 168 us for either, forward of 2,097,152 rows
+// of 64 -> 128 -> 48).
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
@@ -234,7 +236,8 @@ __device__ __forceinline__ void round_pair(float a, float b, uint32_t& hi, uint3
 // The special-function unit (16 results a cycle and SM) takes two operations a
 // value. One reciprocal for two values, 1 / a = b / (a b), saves a quarter of
 // them but costs as much again in products and moves: 196 against 168 us for
-// 2,097,152 rows of 64 -> 128 -> 48, and 168 with it for every second pair.
+// 2,097,152 rows of 64 -> 128 -> 48 with hidden values of one part, and 168 with
+// it for every second pair.
 template <int kW>
 __device__ __forceinline__ void gate(const float (&g)[kW], const float (&u)[kW],
                                      uint32_t (&h)[kW / 2], uint32_t (&lo)[kW / 2]) {

@@ -19,8 +19,8 @@
 // nearest. Bound: the matrix instructions, 24 to a stage, and what stands
 // before a tile's first and after its last: 50,000 rows of 256 -> 512 -> 256
 // forward 390 us (605 TFLOP/s of bf16 products), backward 1344 us. Parts of
-// values below 2^-100 fall out of bf16's range, and an infinity's further parts
-// are NaN.
+// values below 2^-100 fall out of bf16's range, and the further parts of an
+// infinity, or of a value that rounds to one in bf16 (from 3.396e38 on), are NaN.
 #include "tgs_ffn.cuh"
 #include "tgs_tc.cuh"
 

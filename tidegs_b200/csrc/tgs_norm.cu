@@ -161,9 +161,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_kernel(const NormParams
 }
 
 // Blocks to an SM that the compiler has to leave registers for (0: it chooses).
-// Rows of many values to a thread are held back by too few of them: 100,003
-// rows of 768 bf16 (24 values) 138 us with two, 185 with the one that it chose;
-// 300,000 of 301 fp32 (16) 522 against 698; the others lose by it.
+// Rows of many values to a thread are held back by too few of them. 200 MB in
+// each tensor, us with this rule and with its own choice, by type and columns:
+//   16 values, two blocks: bf16 64, 256, 512 as they were (155, 168, 177); single
+//      loads, fp32 257, 301, 511 329, 298, 235 (436, 394, 292), bf16 301, 509
+//      690, 480 (873, 557)
+//   24 values, two: bf16 520, 640, 768 233, 196, 171 (320, 271, 232)
+//   32 values, one: bf16 1024 206 (238); two blocks 348
+// Fewer values, and rows that a block shares, have registers for more anyway.
 constexpr int norm_min_blocks(int values, bool block) {
   return block || values < 16 ? 0 : values <= 24 ? 2 : 1;
 }
@@ -349,7 +354,10 @@ int launch_norm(NormParams p, cudaStream_t s, int* blocks) {
 // kNv and kU: few threads to a row, for few exchanges (at 59 columns of fp32,
 // 8 threads of 8 values against 32 of 2), while a thread keeps about 64 bytes
 // of each of its tensors on their way and no more values than its registers
-// hold (the backward has four sets).
+// hold (the backward has four sets). Three vectors a thread, of a warp to the row,
+// against four: bf16 520, 640 and 768 columns backward 233, 196 and 171 us of
+// 334, 281 and 240, fp32 260, 320 and 384 146, 127 and 113 of 169, 145 and 129,
+// forward 78, 69 and 68 of 87, 79 and 72 (200 MB in each tensor).
 template <class T, int kVec, bool kBwd>
 int launch_norm_vec(const NormParams& p, cudaStream_t s, int* blocks) {
   constexpr int kWarp = 32 * kVec, kWide = kNormThreads * kVec;  // values of one load
@@ -363,9 +371,7 @@ int launch_norm_vec(const NormParams& p, cudaStream_t s, int* blocks) {
   } else {
     if (c <= 4 * kVec) return launch_norm<T, kVec, 1, kBwd ? 2 : 4, false, kBwd>(p, s, blocks);
     if (c <= 2 * kWarp) return launch_norm<T, kVec, 2, kBwd ? 1 : 2, false, kBwd>(p, s, blocks);
-    if constexpr (sizeof(T) == 2) {
-      if (c <= 3 * kWarp) return launch_norm<T, kVec, 3, 1, false, kBwd>(p, s, blocks);
-    }
+    if (c <= 3 * kWarp) return launch_norm<T, kVec, 3, 1, false, kBwd>(p, s, blocks);
     if (c <= 4 * kWarp) return launch_norm<T, kVec, 4, 1, false, kBwd>(p, s, blocks);
     if (c <= kWide) return launch_norm<T, kVec, 1, 4, true, kBwd>(p, s, blocks);
     if (c <= 2 * kWide) return launch_norm<T, kVec, 2, 2, true, kBwd>(p, s, blocks);
