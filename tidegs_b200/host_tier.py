@@ -498,14 +498,28 @@ class PinnedBlockCache:
         return ptrs, rows
 
     # -- lookups and single-flight reads -------------------------------------
-    def _lookup_cached_or_flushing(self, block_id: int, promote_flushing: bool = False):
+    def _hold(self, entry: Optional[int], held: Optional[List[int]]) -> None:
+        """One more reference on the entry, kept in `held` (caller holds
+        cache_lock)."""
+        if held is not None and entry is not None:
+            self._refs[entry] += 1
+            held.append(entry)
+
+    def _lookup_cached_or_flushing(self, block_id: int, promote_flushing: bool = False,
+                                   held: Optional[List[int]] = None):
+        """(view, where) of a block at hand, or (None, None). With `held`, its
+        entry gets a reference, so that a flush or an eviction does not hand it
+        to another block while the caller still gathers its own."""
         with self.cache_lock:
             t = self.cache_data.get(block_id)
             if t is not None:
                 self.cache_data.move_to_end(block_id)
+                self._hold(self._cache_entry.get(block_id), held)
                 return t, "cache"
-        with self.flushing_lock:
-            entry = self.flushing_buffer.get(block_id)
+            with self.flushing_lock:
+                entry = self.flushing_buffer.get(block_id)
+                if entry is not None:
+                    self._hold(self._flush_entry.get(block_id), held)
         if entry is None:
             return None, None
         t = entry[0]
@@ -597,12 +611,12 @@ class PinnedBlockCache:
         return (view.data_ptr() - self.slab.data_ptr()) // self._entry_bytes
 
     def _read_claimed_blocks(self, block_ids: List[int], result: Dict[int, torch.Tensor],
-                             cache_hits: List[int]) -> Tuple[int, float]:
+                             cache_hits: List[int], held: List[int]) -> Tuple[int, float]:
         if not block_ids:
             return 0, 0.0
         to_read, resolved = [], []
         for b in block_ids:
-            t, source = self._lookup_cached_or_flushing(b)
+            t, source = self._lookup_cached_or_flushing(b, held=held)
             if t is not None:
                 result[b] = t
                 cache_hits.append(b)
@@ -619,6 +633,7 @@ class PinnedBlockCache:
             with self.cache_lock:
                 for b in loaded:
                     result[b] = self.cache_data[b]
+                    self._hold(self._cache_entry.get(b), held)
             return len(to_read), time.time() - t0
         finally:
             self._complete_inflight_reads(to_read)
@@ -903,6 +918,19 @@ class PinnedBlockCache:
         buffer, then a read another caller has in flight, then the block log
         (tiered_cache_manager.py:637-732)."""
         result: Dict[int, torch.Tensor] = {}
+        held: List[int] = []
+        try:
+            self._gather(needed_block_ids, result, held)
+        finally:
+            with self.cache_lock:
+                for e in held:
+                    self._release(e)
+        self._maybe_evict()
+        return result
+
+    def _gather(self, needed_block_ids: List[int], result: Dict[int, torch.Tensor],
+                held: List[int]) -> None:
+        """prefetch's reads; the entries of `result` are held."""
         cache_hits: List[int] = []
         read_ids: List[int] = []
         waits = []
@@ -913,7 +941,7 @@ class PinnedBlockCache:
             if b in seen:
                 continue
             seen.add(b)
-            t, source = self._lookup_cached_or_flushing(b)
+            t, source = self._lookup_cached_or_flushing(b, held=held)
             if t is not None:
                 result[b] = t
                 cache_hits.append(b)
@@ -923,12 +951,12 @@ class PinnedBlockCache:
                 read_ids.append(b)
             else:
                 waits.append((b, ev))
-        reads, read_time = self._read_claimed_blocks(read_ids, result, cache_hits)
+        reads, read_time = self._read_claimed_blocks(read_ids, result, cache_hits, held)
         while waits:
             fallback, again = [], []
             for b, ev in waits:
                 self._wait_for_inflight_read(ev)
-                t, source = self._lookup_cached_or_flushing(b)
+                t, source = self._lookup_cached_or_flushing(b, held=held)
                 if t is not None:
                     result[b] = t
                     cache_hits.append(b)
@@ -939,7 +967,7 @@ class PinnedBlockCache:
                     self.stats["inflight_fallback_blocks"] += 1
                 else:
                     again.append((b, ev2))
-            n, dt = self._read_claimed_blocks(fallback, result, cache_hits)
+            n, dt = self._read_claimed_blocks(fallback, result, cache_hits, held)
             reads += n
             read_time += dt
             waits = again
@@ -948,8 +976,6 @@ class PinnedBlockCache:
         self.stats["urgent_prefetch_time"] += read_time
         self.stats["cache_hits"] += len(cache_hits)
         self.stats["cache_misses"] += reads
-        self._maybe_evict()
-        return result
 
     def prefetch_future(self, block_ids: List[int]) -> int:
         """Queues not-yet-cached blocks for the background reader
